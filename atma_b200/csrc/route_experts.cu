@@ -1,0 +1,378 @@
+// Which experts a token goes to, with what weights, and the tokens in the order of their experts.
+//
+//   score = sigmoid(z) or softmax(z);  key = score + bias;  a group's key = the sum of its two best keys
+//   the best groups stay; of their experts the k with the largest keys, falling, the lower index first where keys are equal
+//   weight = score (/ the sum over the k) * scale
+//
+// A choice is only as good as the difference between the keys that it turns on, and fp32 keys are off by some 1e-7.  So a warp takes
+// a token in fp32 first, and where two neighbours among the sorted best (and the first one left out, and the groups likewise) are
+// nearer to one another than their errors can reach, it takes the token again with keys in fp64: one token in some hundreds.  Without a
+// bias and groups both scores grow with the logit, which is then the key itself and exact.
+//
+// A warp holds a token's experts, V of them a lane, neighbours in neighbouring places.  Largest values come by redux over the keys as
+// ordered integers.  A NaN counts as the smallest logit, so that every choice is an expert; infinities as the largest finite values.
+//
+// The order: a CTA's tokens are a chunk; it leaves how many of them go to every expert (route), and a second launch adds up the chunks in
+// front and gives every (token, choice) its place among its expert's, by counts and ranks alone (order): the same result at every run.
+// One chunk does both in the first launch.
+#include "common.cuh"
+#include "early.cuh"
+#include "../../include/atma_decoder.h"
+
+#include <cfloat>
+
+namespace atma {
+
+namespace {
+
+constexpr int kRouteThreads = 1024, kRouteWarps = kRouteThreads / 32;
+constexpr int kMaxExperts = 512;
+constexpr float kKeyError = 4e-6f;          // twice what fp32 scores and their sum with a bias are off by, relative to |key| + 1
+
+struct RouteArgs {
+  const float* logits; int64_t l_rs;
+  const float* bias;
+  int32_t* ids;
+  float* weights;
+  int32_t* counts;                          // [chunks][experts]
+  int32_t *order, *place, *starts;
+  int tokens, experts, k, groups, top_groups, chunk, chunks;
+  float scale;
+  bool sigmoid, renormalize;
+};
+
+// floats and doubles as integers in the same order; 0 is below all of them
+__device__ __forceinline__ uint32_t ordered(float f) {
+  const uint32_t u = __float_as_uint(f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t ordered(double f) {
+  const uint64_t u = (uint64_t)__double_as_longlong(f);
+  return u >> 63 ? ~u : u | (1ull << 63);
+}
+__device__ __forceinline__ float value_of(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u); }
+__device__ __forceinline__ double value_of(uint64_t u) { return __longlong_as_double((long long)(u >> 63 ? u & ~(1ull << 63) : ~u)); }
+__device__ __forceinline__ uint32_t warp_most(uint32_t u) { return __reduce_max_sync(0xffffffffu, u); }
+__device__ __forceinline__ uint64_t warp_most(uint64_t u) {
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(u >> 32));
+  return (uint64_t)hi << 32 | __reduce_max_sync(0xffffffffu, (uint32_t)(u >> 32) == hi ? (uint32_t)u : 0u);
+}
+
+template <typename F> struct Ordered;
+template <> struct Ordered<float> { using type = uint32_t; };
+template <> struct Ordered<double> { using type = uint64_t; };
+
+__device__ __forceinline__ float exp_of(float x) { return expf(x); }
+__device__ __forceinline__ double exp_of(double x) { return exp(x); }
+
+template <typename F>
+__device__ __forceinline__ F warp_add(F v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// The scores of a lane's experts.
+template <typename F, int V>
+__device__ __forceinline__ void scores_of(const float (&z)[V], int e0, int experts, bool sigmoid, F (&s)[V]) {
+  if (sigmoid) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) s[v] = F(1) / (F(1) + exp_of(-F(z[v])));
+    return;
+  }
+  float m = -FLT_MAX;
+#pragma unroll
+  for (int v = 0; v < V; ++v) m = fmaxf(m, z[v]);            // behind the last expert z is -FLT_MAX
+  m = value_of(warp_most(ordered(m)));
+  F sum = 0;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    s[v] = e0 + v < experts ? exp_of(F(z[v]) - F(m)) : F(0);
+    sum += s[v];
+  }
+  sum = warp_add(sum);
+#pragma unroll
+  for (int v = 0; v < V; ++v) s[v] /= sum;
+}
+
+// Takes experts out whose group is not among the best; false where fp32 keys do not settle which those are.
+template <typename F, int V>
+__device__ __forceinline__ bool keep_groups(typename Ordered<F>::type (&key)[V], int e0, const RouteArgs& a) {
+  using U = typename Ordered<F>::type;
+  const int lane = threadIdx.x & 31, size = a.experts / a.groups;
+  U mine[2] = {0, 0};                                        // keys of groups `lane` and `lane + 32`
+  for (int g = 0; g < a.groups; ++g) {
+    U best = 0, second = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const U u = e0 + v >= g * size && e0 + v < (g + 1) * size ? key[v] : U(0);
+      second = u > best ? best : (u > second ? u : second);
+      best = u > best ? u : best;
+    }
+    const U most = warp_most(best);
+    const uint32_t holders = __ballot_sync(0xffffffffu, best == most);
+    const U next = warp_most(lane == __ffs(holders) - 1 ? second : best);
+    const F sum = next == 0 ? value_of(most) : value_of(most) + value_of(next);      // a group of one expert has no second
+    if (lane == (g & 31)) mine[g >> 5] = ordered(sum);
+  }
+  uint64_t left = 0;
+  U last = 0;
+  bool settled = true;
+  for (int n = 0; n <= a.top_groups && n < a.groups; ++n) {
+    const U most = warp_most(mine[0] > mine[1] ? mine[0] : mine[1]);
+    const uint32_t low = __ballot_sync(0xffffffffu, mine[0] == most), high = __ballot_sync(0xffffffffu, mine[1] == most);
+    const int g = low ? __ffs(low) - 1 : 31 + __ffs(high);
+    if (n == a.top_groups) {                                 // the best one that goes: too near to the last that stays?
+      if constexpr (std::is_same<F, float>::value) {
+        const float p = value_of(last), q = value_of(most);
+        settled = p - q > 2.f * kKeyError * (fabsf(p) + 1.f);
+      }
+      break;
+    }
+    last = most;
+    left |= 1ull << g;
+    if (lane == (g & 31)) mine[g >> 5] = 0;
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    if (e0 + v < a.experts && !(left >> ((e0 + v) / size) & 1)) key[v] = ordered(-F(INFINITY));
+  return settled;
+}
+
+// The k best of a token: lane j < 32 keeps choice j (and choice j + 32 in the second place).  False where fp32 keys do not settle them.
+template <typename F, int V, bool kExact>
+__device__ __forceinline__ bool choose(const float (&z)[V], int e0, const RouteArgs& a, int (&id)[2], float (&score)[2]) {
+  using U = typename Ordered<F>::type;
+  const int lane = threadIdx.x & 31;
+  F s[V];
+  U key[V];
+  scores_of<F, V>(z, e0, a.experts, a.sigmoid, s);
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int e = e0 + v;
+    F f = kExact ? F(z[v]) : s[v];
+    if (!kExact && a.bias != nullptr && e < a.experts) {
+      const float b = a.bias[e];
+      f += F(isnan(b) ? -INFINITY : b);
+    }
+    key[v] = e < a.experts ? ordered(f) : U(0);
+  }
+  bool settled = true;
+  if (!kExact && a.groups > 1) settled = keep_groups<F, V>(key, e0, a);
+  U last = 0;
+  const bool check = std::is_same<F, float>::value && !kExact;
+  const int rounds = check && a.k < a.experts ? a.k + 1 : a.k;
+  for (int n = 0; n < rounds; ++n) {
+    U best = 0;
+    F at = 0;
+    int where = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (key[v] > best) { best = key[v]; at = s[v]; where = v; }
+    const U most = warp_most(best);
+    if (check && n > 0) {
+      const float p = (float)value_of(last), q = (float)value_of(most);
+      settled = settled && p - q > kKeyError * (fabsf(p) + 1.f);       // also where both are -inf
+    }
+    last = most;
+    if (n == a.k) break;
+    const int holder = __ffs(__ballot_sync(0xffffffffu, best == most)) - 1;
+    const int e = __shfl_sync(0xffffffffu, e0 + where, holder);
+    const float got = (float)__shfl_sync(0xffffffffu, at, holder);
+    if (lane == (n & 31)) { id[n >> 5] = e; score[n >> 5] = got; }
+    if (lane == holder) {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (v == where) key[v] = 0;
+    }
+  }
+  return settled;
+}
+
+template <int V>
+__device__ __noinline__ void choose_in_64(const float (&z)[V], int e0, const RouteArgs& a, int (&id)[2], float (&score)[2]) {
+  choose<double, V, false>(z, e0, a, id, score);
+}
+
+// ---- places ----------------------------------------------------------------------------------------------
+struct OrderShared {
+  int32_t base[kMaxExperts];                // the next place of every expert
+  int32_t scan[kRouteWarps];
+  uint16_t counts[kRouteWarps][kMaxExperts];
+};
+
+// Sum over the threads in front of this one.
+__device__ __forceinline__ int scan_exclusive(int v, int32_t* s_scan, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int in = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, in, o);
+    if (lane >= o) in += t;
+  }
+  if (lane == 31) s_scan[warp] = in;
+  __syncthreads();
+  int before = 0, all = 0;
+  for (int w = 0; w < kRouteWarps; ++w) {
+    if (w < warp) before += s_scan[w];
+    all += s_scan[w];
+  }
+  __syncthreads();
+  *total = all;
+  return before + in - v;
+}
+
+// Places of the entries of tokens [t0, t1): `before` and `total` are thread e's counts of expert e in the chunks in front and in all.
+__device__ void place_entries(OrderShared& s, const RouteArgs& a, int t0, int t1, int before, int total, bool write_starts) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int all;
+  const int start = scan_exclusive(total, s.scan, &all);
+  if (tid < a.experts) {
+    s.base[tid] = start + before;
+    if (write_starts) a.starts[tid] = start;
+  }
+  if (write_starts && tid == 0) a.starts[a.experts] = all;
+  const int first = t0 * a.k, entries = t1 * a.k;
+  for (int i0 = first; i0 < entries; i0 += kRouteThreads) {
+    for (int e = lane; e < a.experts; e += 32) s.counts[warp][e] = 0;
+    __syncthreads();                                         // base is there too
+    const int i = i0 + tid;
+    const int e = i < entries ? a.ids[i] : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, e);
+    const int rank = __popc(same & ((1u << lane) - 1));
+    if (e >= 0 && rank == 0) s.counts[warp][e] = (uint16_t)__popc(same);
+    __syncthreads();
+    int batch = 0;                                           // thread e's: the batch's entries of expert e
+    if (tid < a.experts)
+      for (int w = 0; w < kRouteWarps; ++w) {                // counts become the warps' first places
+        const int n = s.counts[w][tid];
+        s.counts[w][tid] = (uint16_t)batch;
+        batch += n;
+      }
+    __syncthreads();
+    if (e >= 0) {
+      const int at = s.base[e] + s.counts[warp][e] + rank;
+      a.order[at] = i;
+      a.place[i] = at;
+    }
+    __syncthreads();
+    if (tid < a.experts) s.base[tid] += batch;
+  }
+}
+
+template <int V>
+__global__ void __launch_bounds__(kRouteThreads)
+route_experts_kernel(const RouteArgs a) {
+  early_start();
+  __shared__ int32_t s_counts[kMaxExperts];
+  extern __shared__ uint8_t s_more[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, e0 = lane * V;
+  for (int e = tid; e < a.experts; e += kRouteThreads) s_counts[e] = 0;
+  __syncthreads();
+  const int t0 = blockIdx.x * a.chunk, t1 = min(a.tokens, t0 + a.chunk);
+  for (int t = t0 + warp; t < t1; t += kRouteWarps) {
+    const float* row = a.logits + (int64_t)t * a.l_rs;
+    float z[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float f = e0 + v < a.experts ? row[e0 + v] : -FLT_MAX;
+      z[v] = fminf(fmaxf(f, -FLT_MAX), FLT_MAX);             // a NaN becomes -FLT_MAX here
+    }
+    int id[2] = {0, 0};
+    float score[2] = {0.f, 0.f};
+    if (a.bias == nullptr && a.groups == 1) choose<float, V, true>(z, e0, a, id, score);
+    else if (!choose<float, V, false>(z, e0, a, id, score)) choose_in_64<V>(z, e0, a, id, score);
+    if (a.renormalize) {
+      const float sum = warp_sum(score[0] + score[1]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) score[i] = sum > 0.f ? score[i] / sum : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (lane + 32 * i < a.k) {
+        a.ids[(int64_t)t * a.k + lane + 32 * i] = id[i];
+        a.weights[(int64_t)t * a.k + lane + 32 * i] = score[i] * a.scale;
+        atomicAdd(&s_counts[id[i]], 1);                      // whole numbers: any order gives the same
+      }
+  }
+  __syncthreads();
+  if (a.chunks == 1) {
+    const int n = tid < a.experts ? s_counts[tid] : 0;
+    place_entries(*reinterpret_cast<OrderShared*>(s_more), a, t0, t1, 0, n, true);
+  } else {
+    for (int e = tid; e < a.experts; e += kRouteThreads) a.counts[(int64_t)blockIdx.x * a.experts + e] = s_counts[e];
+  }
+}
+
+__global__ void __launch_bounds__(kRouteThreads)
+order_experts_kernel(const RouteArgs a) {
+  extern __shared__ uint8_t s_more[];
+  const int tid = threadIdx.x;
+  int before = 0, total = 0;
+  if (tid < a.experts) {
+#pragma unroll 8
+    for (int c = 0; c < a.chunks; ++c) {
+      const int n = a.counts[(int64_t)c * a.experts + tid];
+      if (c < (int)blockIdx.x) before += n;
+      total += n;
+    }
+  }
+  const int t0 = blockIdx.x * a.chunk;
+  place_entries(*reinterpret_cast<OrderShared*>(s_more), a, t0, min(a.tokens, t0 + a.chunk), before, total, blockIdx.x == 0);
+}
+
+// Tokens of a chunk: as few as give every SM one, 32 at least.
+int route_chunk(int tokens) {
+  const int sms = sm_count_of_current_device(), n = (tokens + sms - 1) / sms;
+  return n <= 32 ? 32 : (n + 31) / 32 * 32;
+}
+
+template <int V>
+int launch_route(const RouteArgs& a, cudaStream_t st) {
+  auto kernel = route_experts_kernel<V>;
+  const size_t more = a.chunks == 1 ? sizeof(OrderShared) : 0;
+  launch_early(a.tokens, kernel, a.chunks, kRouteThreads, more, st, a);
+  return launch_status("route_experts");
+}
+
+}  // namespace
+}  // namespace atma
+
+using namespace atma;
+
+extern "C" int64_t atma_route_scratch_ints(int tokens, int experts) {
+  if (tokens <= 0 || experts <= 0) return 0;
+  const int chunk = route_chunk(tokens), chunks = (tokens + chunk - 1) / chunk;
+  return chunks == 1 ? 0 : (int64_t)chunks * experts;
+}
+
+extern "C" int atma_route_experts(const float* logits, int64_t l_rs, const float* bias, int32_t* ids, float* weights, int32_t* order,
+                                  int32_t* place, int32_t* starts, int32_t* scratch, int tokens, int experts, int k, int sigmoid,
+                                  int groups, int top_groups, int renormalize, float scale, void* stream) {
+  ATMA_REQUIRE(experts > 0 && experts <= kMaxExperts, "route_experts: %d experts, at most %d are served", experts, kMaxExperts);
+  ATMA_REQUIRE(tokens >= 0 && k > 0 && (int64_t)tokens * k <= INT32_MAX - kRouteThreads, "route_experts: bad shape");
+  ATMA_REQUIRE(groups > 0 && groups <= 64 && experts % groups == 0 && top_groups > 0 && top_groups <= groups,
+               "route_experts: %d of %d groups of %d experts", top_groups, groups, experts);
+  ATMA_REQUIRE(k <= 64 && k <= experts / groups * top_groups, "route_experts: %d experts of %d", k, experts / groups * top_groups);
+  ATMA_REQUIRE(starts != nullptr, "route_experts: null tensors");
+  cudaStream_t st = (cudaStream_t)stream;
+  if (tokens == 0) {
+    ATMA_CUDA_OK(cudaMemsetAsync(starts, 0, (experts + 1) * sizeof(int32_t), st));
+    return ATMA_OK;
+  }
+  ATMA_REQUIRE(logits != nullptr && ids != nullptr && weights != nullptr && order != nullptr && place != nullptr && l_rs >= experts,
+               "route_experts: null tensors or overlapping rows");
+  const int chunk = route_chunk(tokens), chunks = (tokens + chunk - 1) / chunk;
+  ATMA_REQUIRE(chunks == 1 || scratch != nullptr, "route_experts: no scratch memory");
+  const RouteArgs a{logits, l_rs, bias, ids, weights, scratch, order, place, starts, tokens, experts, k, groups, top_groups, chunk, chunks, scale,
+                    sigmoid != 0, renormalize != 0};
+  int rc;
+  if (experts <= 32) rc = launch_route<1>(a, st);
+  else if (experts <= 64) rc = launch_route<2>(a, st);
+  else if (experts <= 128) rc = launch_route<4>(a, st);
+  else if (experts <= 256) rc = launch_route<8>(a, st);
+  else rc = launch_route<16>(a, st);
+  if (rc != ATMA_OK || chunks == 1) return rc;
+  order_experts_kernel<<<chunks, kRouteThreads, sizeof(OrderShared), st>>>(a);
+  return launch_status("order_experts");
+}

@@ -1,0 +1,92 @@
+"""Mixtures of experts (libatma_decoder.so): which experts a token goes to, and their feed-forwards in 8 bits.
+
+    routes = route_experts(logits, top_k, score="sigmoid", bias=balance, groups=8, top_groups=4)
+    y = expert_mlp(rows, w_gate_up, w_down, routes)
+
+All launches have shapes that the host knows (tokens x top_k rows), so that a step with experts can be captured in a CUDA graph.
+"""
+
+import torch
+
+from . import _lib
+from .decoder_ops import _check
+from .fp8_ops import Fp8Rows, Fp8Weight, _here, _new_rows, _product, _row_stride, _scale_stride, _TYPES
+
+MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 512, 64, 64
+
+
+class Routes:
+    """Where tokens go.  ids, weights (tokens, top_k): experts (int32) and their weights (float32), the best first.  A pair
+    token * top_k + choice is a row of the experts' products: order[row] = pair (rows by expert, then by pair), place[pair] = row,
+    and expert e's rows are starts[e] .. starts[e + 1] - 1 (all int32)."""
+
+    __slots__ = ("ids", "weights", "order", "place", "starts", "experts")
+
+    def __init__(self, ids, weights, order, place, starts):
+        self.ids, self.weights, self.order, self.place, self.starts, self.experts = ids, weights, order, place, starts, starts.shape[0] - 1
+
+
+def route_experts(logits, top_k, *, score="softmax", bias=None, groups=1, top_groups=None, renormalize=True, scale=1.0):
+    """Experts of tokens by their logits (tokens, experts).  ``score``: "softmax" or "sigmoid"; a choice goes by score + ``bias``
+    (experts,) float32, weights by the scores alone.  ``groups``: of so many groups of neighbouring experts only ``top_groups`` are
+    looked at, those with the largest sum of their two best (None: all).  ``renormalize``: a token's weights are divided by their sum (zero where that is
+    zero); ``scale`` multiplies them.  Equal ones: the lower index first.  NaN and -inf count as the least finite logit, inf as the
+    largest; a choice is decided as in 64-bit arithmetic."""
+    _here(logits, bias)
+    if logits.ndim != 2 or not logits.is_floating_point():
+        raise ValueError("logits must be a (tokens, experts) matrix")
+    (tokens, experts), dev = logits.shape, logits.device
+    top_groups = groups if top_groups is None else top_groups
+    if score not in ("softmax", "sigmoid"):
+        raise ValueError(f"unknown score {score!r}; expected 'softmax' or 'sigmoid'")
+    if not 0 < experts <= MAX_EXPERTS or not 0 < groups <= MAX_GROUPS or experts % groups or not 0 < top_groups <= groups:
+        raise ValueError(f"{top_groups} of {groups} groups of {experts} experts (at most {MAX_EXPERTS} in {MAX_GROUPS} groups)")
+    if not 0 < top_k <= min(MAX_TOP_K, experts // groups * top_groups):
+        raise ValueError(f"{top_k} of {experts // groups * top_groups} experts (at most {MAX_TOP_K})")
+    if logits.dtype != torch.float32 or logits.stride(1) != 1 and experts > 1 or logits.stride(0) < experts and tokens > 1:
+        logits = logits.float().contiguous()
+    if bias is not None:
+        if bias.shape != (experts,):
+            raise ValueError(f"bias must have {experts} values, not the shape {tuple(bias.shape)}")
+        bias = bias.float().contiguous()
+    lib, n = _lib.load_decoder(), tokens * top_k
+    ids, weights = torch.empty((tokens, top_k), device=dev, dtype=torch.int32), torch.empty((tokens, top_k), device=dev)
+    order, place = torch.empty(n, device=dev, dtype=torch.int32), torch.empty(n, device=dev, dtype=torch.int32)
+    starts = torch.empty(experts + 1, device=dev, dtype=torch.int32)
+    ints = lib.atma_route_scratch_ints(tokens, experts)
+    scratch = torch.empty(ints, device=dev, dtype=torch.int32) if ints else None
+    _check(lib.atma_route_experts(logits.data_ptr(), logits.stride(0) if tokens > 1 else experts, None if bias is None else bias.data_ptr(), ids.data_ptr(),
+                                  weights.data_ptr(), order.data_ptr(), place.data_ptr(), starts.data_ptr(), None if scratch is None else scratch.data_ptr(),
+                                  tokens, experts, top_k, score == "sigmoid", groups, top_groups, bool(renormalize), scale, _lib.stream_ptr()))
+    return Routes(ids, weights, order, place, starts)
+
+
+def expert_mlp(x, w_gate_up, w_down, routes, add=None, dtype=torch.bfloat16):
+    """Gelu-gated feed-forwards of the tokens' experts, weighted and summed: sum over j of weights[t, j] * down(gelu_tanh(gate x_t) * up x_t).
+    x: Fp8Rows (tokens, width); w_gate_up (experts, 2, ff, width), w_down (experts, width, ff): Fp8Weight; the activations between them go
+    to 8 bits like any rows.  ``add`` (tokens, width) is added.  Returns (tokens, width) in ``dtype``, bfloat16 or float32; an expert's
+    results are in that type too before they are summed, in fp32."""
+    if not isinstance(x, Fp8Rows) or not isinstance(w_gate_up, Fp8Weight) or not isinstance(w_down, Fp8Weight) or not isinstance(routes, Routes):
+        raise ValueError("expert_mlp takes Fp8Rows, two Fp8Weights and Routes")
+    (tokens, width), experts, top_k = x.shape, routes.experts, routes.ids.shape[1]
+    ff = w_down.shape[-1]
+    if w_gate_up.shape != (experts, 2, ff, width) or w_down.shape != (experts, width, ff) or routes.ids.shape[0] != tokens:
+        raise ValueError(f"weights of the shapes {tuple(w_gate_up.shape)} and {tuple(w_down.shape)} do not fit rows {tuple(x.shape)} and "
+                         f"{tuple(routes.ids.shape)} choices of {experts} experts")
+    if dtype not in _TYPES or add is not None and (add.shape != x.shape or add.dtype != dtype or not add.is_contiguous()):
+        raise ValueError("bfloat16 or float32, add contiguous in the same type")
+    _here(x.values, w_gate_up.values, w_down.values, routes.ids, add)
+    lib, n, dev = _lib.load_decoder(), tokens * top_k, x.values.device
+    out = torch.empty((tokens, width), device=dev, dtype=dtype)
+    if tokens == 0:
+        return out
+    mine = _new_rows(n, width, dev)
+    _check(lib.atma_scatter_rows_fp8(x.values.data_ptr(), _row_stride(x.values), x.scales.data_ptr(), _scale_stride(x.scales), routes.place.data_ptr(), top_k,
+                                     mine.values.data_ptr(), _row_stride(mine.values), mine.scales.data_ptr(), n, tokens, width, _lib.stream_ptr()))
+    z = _product(mine, w_gate_up, torch.empty((n, 2 * ff), device=dev), routes.starts, experts, 2)
+    act = _new_rows(n, ff, dev)
+    _check(lib.atma_gelu_gate_fp8(z.data_ptr(), z.stride(0), act.values.data_ptr(), _row_stride(act.values), act.scales.data_ptr(), n, n, ff, _lib.stream_ptr()))
+    y = _product(act, w_down, torch.empty((n, width), device=dev, dtype=dtype), routes.starts, experts)
+    _check(lib.atma_combine_experts(y.data_ptr(), routes.place.data_ptr(), routes.weights.data_ptr(), None if add is None else add.data_ptr(), out.data_ptr(),
+                                    tokens, top_k, width, _lib.DTYPE_CODE[dtype], _lib.stream_ptr()))
+    return out

@@ -1,0 +1,220 @@
+"""Rows and weights in 8 bits (libatma_decoder.so): what a layer multiplies, in e4m3 with fp32 scales.
+
+A row has a scale for every block of 128 channels: s = max(max |x| / 448, 2^-126), values = e4m3(x / s), the quotient rounded once.
+A weight has one for every block of 128 rows and 128 columns.  A NaN or an infinity in a row makes the row's results NaN, and no
+other's.  Everything launches on the current CUDA stream, allocates only its results and never synchronises.
+"""
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .decoder_ops import _check
+
+BLOCK = 128                           # channels that share a scale
+TOP, LEAST = 448.0, 2.0 ** -126       # the largest e4m3 value, the smallest scale
+E4M3 = torch.float8_e4m3fn
+_TYPES = (torch.bfloat16, torch.float32)
+
+
+def blocks(n):
+    return -(-n // BLOCK)
+
+
+def _here(*tensors):
+    """All of them on the current CUDA device; launches go to its current stream."""
+    for t in tensors:
+        if t is not None:
+            if not t.is_cuda:
+                raise RuntimeError("operations in 8 bits require CUDA tensors (atma_b200 has no CPU path)")
+            if t.device.index != torch._C._cuda_getDevice():
+                raise ValueError(f"a tensor on {t.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+
+
+def _storage(shape, width, device):
+    """Rows of ``width`` bytes that start on 16-byte boundaries."""
+    pad = -width % 16
+    return torch.empty((*shape, width + pad), device=device, dtype=E4M3)[..., :width] if pad else torch.empty((*shape, width), device=device, dtype=E4M3)
+
+
+def _on_16_bytes(values):
+    """Whether the rows of (..., rows, width) lie dense behind one another on 16-byte boundaries."""
+    width, step = values.shape[-1], values.stride(-2)
+    if values.stride(-1) != 1 and width > 1 or values.data_ptr() % 16:
+        return False
+    if values.numel() == width:                                                    # one row: its stride is not used
+        return True
+    if step % 16 or step < width:
+        return False
+    for d in range(values.ndim - 3, -1, -1):
+        step *= values.shape[d + 1]
+        if values.shape[d] > 1 and values.stride(d) != step:
+            return False
+    return True
+
+
+def _row_stride(values):
+    return values.stride(-2) if values.numel() != values.shape[-1] else -(-values.shape[-1] // 16) * 16
+
+
+class Fp8Rows:
+    """Rows in 8 bits: ``values`` (rows, width) float8_e4m3fn, ``scales`` (rows, blocks) float32.  Rows that do not start on 16-byte
+    boundaries and scales that do not lie block by block (stride 1 along the rows) are copied."""
+
+    __slots__ = ("values", "scales")
+
+    def __init__(self, values, scales):
+        if values.ndim != 2 or values.dtype != E4M3 or scales.dtype != torch.float32 or scales.shape != (values.shape[0], blocks(values.shape[1])):
+            raise ValueError("rows in 8 bits are (rows, width) float8_e4m3fn values and (rows, blocks of 128) float32 scales")
+        if scales.device != values.device:
+            raise ValueError("values and scales must be on one device")
+        if not _on_16_bytes(values):
+            values = _storage(values.shape[:1], values.shape[1], values.device).copy_(values)
+        if scales.shape[0] > 1 and scales.stride(0) != 1 or scales.shape[1] > 1 and scales.stride(1) < scales.shape[0]:
+            scales = scales.t().contiguous().t()
+        self.values, self.scales = values, scales
+
+    @property
+    def shape(self):
+        return self.values.shape
+
+    def __getitem__(self, rows):
+        """Some of the rows (a slice)."""
+        return Fp8Rows(self.values[rows], self.scales[rows])
+
+    def wide(self):
+        """What the rows stand for, in fp32."""
+        return self.values.float() * self.scales.repeat_interleave(BLOCK, 1)[:, :self.shape[1]]
+
+
+def _scale_stride(scales):
+    """Words between the scales of neighbouring blocks."""
+    return max(scales.stride(1), scales.shape[0]) if scales.shape[1] > 1 else max(scales.shape[0], 1)
+
+
+class Fp8Weight:
+    """A weight in 8 bits: ``values`` (..., N, K) float8_e4m3fn, ``scales`` (..., blocks of N, blocks of K) float32.  Leading dimensions
+    hold matrices of one shape: an expert's, or the gate and the up projection of a feed-forward (2, N, K)."""
+
+    __slots__ = ("values", "scales")
+
+    def __init__(self, values, scales):
+        if values.ndim < 2 or values.dtype != E4M3 or scales.dtype != torch.float32 or \
+                scales.shape != (*values.shape[:-2], blocks(values.shape[-2]), blocks(values.shape[-1])):
+            raise ValueError("a weight in 8 bits is (..., N, K) float8_e4m3fn values and (..., N / 128, K / 128) float32 scales")
+        if scales.device != values.device:
+            raise ValueError("values and scales must be on one device")
+        if not _on_16_bytes(values):
+            values = _storage(values.shape[:-1], values.shape[-1], values.device).copy_(values)
+        self.values, self.scales = values, scales if scales.is_contiguous() else scales.contiguous()
+
+    @classmethod
+    def of(cls, weight):
+        """A weight (..., N, K) in 8 bits (once, when a model is loaded)."""
+        *lead, n, k = weight.shape
+        flat = weight.reshape(-1, n, k)
+        values = _storage((flat.shape[0], n), k, weight.device)
+        scales = torch.empty((flat.shape[0], blocks(n), blocks(k)), device=weight.device)
+        for i, w in enumerate(flat):                                               # one matrix at a time: fp64 copies are large
+            full = torch.zeros((blocks(n) * BLOCK, blocks(k) * BLOCK), device=w.device, dtype=torch.float64)
+            full[:n, :k] = w
+            cells = full.view(blocks(n), BLOCK, blocks(k), BLOCK)
+            s = (cells.abs().amax((1, 3)) / TOP).clamp_min(LEAST).float()
+            q = cells / s[:, None, :, None].double()
+            step = torch.ldexp(torch.ones_like(q), torch.frexp(q).exponent.clamp_min(-5) - 4)     # a conversion would round to fp32 in between
+            values[i].copy_((torch.round(q / step) * step).view_as(full)[:n, :k].to(E4M3))
+            scales[i] = s
+        return cls(values.view(*lead, n, k) if values.is_contiguous() else values.unflatten(0, lead) if lead else values[0], scales.view(*lead, blocks(n), blocks(k)))
+
+    @property
+    def shape(self):
+        return self.values.shape
+
+    def nbytes(self):
+        return self.values.numel() + 4 * self.scales.numel()
+
+    def wide(self):
+        """What the weight stands for, in fp32."""
+        n, k = self.shape[-2:]
+        return self.values.float() * self.scales.repeat_interleave(BLOCK, -2)[..., :n, :].repeat_interleave(BLOCK, -1)[..., :k]
+
+
+def _new_rows(rows, width, device):
+    r = Fp8Rows.__new__(Fp8Rows)
+    r.values, r.scales = _storage((rows,), width, device), torch.empty((blocks(width), rows), device=device).t()
+    return r
+
+
+def quantize_rows(x):
+    """Rows (rows, width) of bfloat16 or float32 in 8 bits."""
+    _here(x)
+    if x.ndim != 2 or x.dtype not in _TYPES or x.shape[1] == 0:
+        raise ValueError("quantize_rows takes a (rows, width) matrix of bfloat16 or float32")
+    if x.stride(1) != 1 and x.shape[1] > 1:
+        x = x.contiguous()
+    n, width = x.shape
+    r = _new_rows(n, width, x.device)
+    _check(_lib.load_decoder().atma_quantize_rows(x.data_ptr(), x.stride(0), r.values.data_ptr(), _row_stride(r.values), r.scales.data_ptr(), max(n, 1), n,
+                                                  width, _lib.DTYPE_CODE[x.dtype], _lib.stream_ptr()))
+    return r
+
+
+def residual_norms_fp8(x, y, weights, eps, offset=1.0, out=None, plain=False):
+    """``decoder_ops.residual_norms`` with results in 8 bits: x + y (x (rows, width) float32; y in the weights' type, or None) goes to
+    ``out`` (None: to x itself); for every weight of ``weights`` (one or two, None = skipped) the normalised row times (offset + weight).
+    Returns [(Fp8Rows, None)], and with ``plain`` the last norm in the weights' type beside its rows in 8 bits."""
+    weights = list(weights)
+    given = [w for w in weights if w is not None]
+    _here(x, y, out, *given)
+    if not given or len(weights) > 2:
+        raise ValueError("one or two norms")
+    dtype, (n, D) = given[0].dtype, x.shape
+    if x.dtype != torch.float32 or not x.is_contiguous() or D == 0:
+        raise ValueError("x must be a contiguous float32 matrix")
+    if dtype not in _TYPES or any(w.dtype != dtype or w.shape != (D,) or not w.is_contiguous() for w in given):
+        raise ValueError(f"weights must have {D} values each and one type, bfloat16 or float32")
+    if y is not None and (y.shape != x.shape or y.dtype != dtype or not y.is_contiguous()):
+        raise ValueError("y must be contiguous, of x's shape and of the weights' type")
+    if out is not None and (out.shape != x.shape or out.dtype != torch.float32 or not out.is_contiguous()):
+        raise ValueError("out must be contiguous, of x's shape and float32")
+    to = out if out is not None else x if y is not None else None
+    rows = [None if w is None else _new_rows(n, D, x.device) for w in weights]
+    h = torch.empty((n, D), device=x.device, dtype=dtype) if plain and weights[-1] is not None else None
+    parts = []
+    for i, (w, r) in enumerate(zip(weights, rows)):
+        parts += (None, None, None, None) if w is None else (w.data_ptr(), r.values.data_ptr(), r.scales.data_ptr(),
+                                                             h.data_ptr() if h is not None and i == len(weights) - 1 else None)
+    if len(weights) == 1:
+        parts += (None, None, None, None)
+    some = next(r for r in rows if r is not None)
+    _check(_lib.load_decoder().atma_residual_norms_fp8(x.data_ptr(), None if y is None else y.data_ptr(), None if to is None else to.data_ptr(), *parts, n, D,
+                                                       _row_stride(some.values), max(n, 1), eps, offset, _lib.DTYPE_CODE[dtype], _lib.stream_ptr()))
+    return [(r, h if i == len(rows) - 1 else None) for i, r in enumerate(rows)]
+
+
+def _product(x, w, out, starts=None, groups=1, parts=1):
+    a = _lib.Fp8Args()
+    a.x, a.x_rs, a.x_scales, a.xs_bs = x.values.data_ptr(), _row_stride(x.values), x.scales.data_ptr(), _scale_stride(x.scales)
+    a.w, a.w_rs, a.w_scales = w.values.data_ptr(), _row_stride(w.values), w.scales.data_ptr()
+    a.out, a.out_rs = out.data_ptr(), out.stride(0) if out.shape[0] > 1 else out.shape[1]
+    a.starts = None if starts is None else starts.data_ptr()
+    a.M, a.N, a.K, a.groups, a.parts, a.dtype = out.shape[0], out.shape[1], x.shape[1], groups, parts, _lib.DTYPE_CODE[out.dtype]
+    _check(_lib.load_decoder().atma_linear_fp8(ctypes.byref(a), _lib.stream_ptr()))
+    return out
+
+
+def linear_fp8(x, weight, out=None, dtype=torch.bfloat16):
+    """x @ weight.T of rows (rows, K) and a weight (N, K) in 8 bits, in ``dtype`` (bfloat16 or float32) or ``out``'s type: sums in fp32,
+    rounded once.  ``out``: (rows, N) with contiguous rows, any row stride."""
+    if not isinstance(x, Fp8Rows) or not isinstance(weight, Fp8Weight) or weight.values.ndim != 2 or weight.shape[1] != x.shape[1] or 0 in weight.shape:
+        raise ValueError("linear_fp8 takes Fp8Rows (rows, K) and an Fp8Weight (N, K)")
+    _here(x.values, weight.values, out)
+    n, N = x.shape[0], weight.shape[0]
+    if out is None:
+        if dtype not in _TYPES:
+            raise ValueError(f"unsupported dtype {dtype}; expected float32 or bfloat16")
+        out = torch.empty((n, N), device=x.values.device, dtype=dtype)
+    elif out.shape != (n, N) or out.dtype not in _TYPES or out.stride(1) != 1 and N > 1 or out.stride(0) < N and n > 1:
+        raise ValueError("out must have the result's shape, contiguous rows and type bfloat16 or float32")
+    return _product(x, weight, out)

@@ -146,6 +146,56 @@ int64_t atma_delta_scan_scratch_bytes(const atma_delta_args* args);
  * `norm_w` [vdim], silu gate; out [n_seqs][H*vdim]. */
 int atma_delta_step(const atma_delta_args* args, const void* norm_w, void* out, int64_t out_rs, float eps, void* stream);
 
+/* ---- rows and weights in 8 bits, experts -------------------------------------------------------------------------
+ * A row in 8 bits: e4m3 values and for every block b of 128 channels an fp32 scale, s = max(max |x| / 448, 2^-126),
+ * q = e4m3(x / s).  Scales lie block by block: scales[b * s_bs + row].  A weight has a scale for every block of 128 rows
+ * and 128 columns, dense [rows / 128][columns / 128].  Rows of values are q_rs bytes apart. */
+
+/* x (rows, width) to 8 bits. */
+int atma_quantize_rows(const void* x, int64_t x_rs, void* q, int64_t q_rs, float* scales, int64_t s_bs, int rows, int width,
+                       int dtype, void* stream);
+
+/* gelu_tanh(z[:, :width]) * z[:, width:] of fp32 rows to 8 bits. */
+int atma_gelu_gate_fp8(const float* z, int64_t z_rs, void* q, int64_t q_rs, float* scales, int64_t s_bs, int rows, int width,
+                       void* stream);
+
+/* atma_residual_norms with results in 8 bits: x + y (y NULL = nothing to add) goes to x_out (NULL = not stored, may be
+ * x); of every non-NULL w the norm goes to q and s and, where h is not NULL, to h in the activation dtype. */
+int atma_residual_norms_fp8(const float* x, const void* y, float* x_out, const void* w1, void* q1, float* s1, void* h1,
+                            const void* w2, void* q2, float* s2, void* h2, int rows, int D, int64_t q_rs, int64_t s_bs,
+                            float eps, float offset, int dtype, void* stream);
+
+/* out[m][n] = sum over b of x_scales[b][m] w_scales[n / 128][b] * (x[m], w[n] over block b), summed in fp32.
+ * groups > 1: the weight holds `groups` matrices of N rows, and rows starts[g] .. starts[g + 1] - 1 of x take the g-th.
+ * parts = 2: a matrix is two of N / 2 rows, each with blocks of its own (scales [groups][parts][..][..]). */
+typedef struct {
+  const void* x; int64_t x_rs; const float* x_scales; int64_t xs_bs;
+  const void* w; int64_t w_rs; const float* w_scales;
+  void* out; int64_t out_rs;         /* dtype ATMA_F32 or ATMA_BF16 */
+  const int32_t* starts;             /* [groups + 1]; NULL = one group of M rows */
+  int M, N, K, groups, parts, dtype;
+} atma_fp8_args;
+int atma_linear_fp8(const atma_fp8_args* args, void* stream);
+
+/* Experts of tokens.  score = sigmoid(logit) or softmax(logits), key = score + bias (NULL = none); of `groups` groups of
+ * neighbouring experts the top_groups with the largest sum of their two largest keys stay; ids [tokens][k]: the k largest
+ * keys of those, falling, lower indices first among equal ones; weights [tokens][k]: their scores, divided by their sum
+ * (renormalize; zero where that is zero), times scale.  NaN and -infinity count as the least finite logit, infinity as
+ * the largest.  order [tokens * k]: token * k + choice of every pair, by expert, then by itself; place: its inverse;
+ * starts [experts + 1]: where every expert's pairs begin.  scratch: atma_route_scratch_ints() words. */
+int atma_route_experts(const float* logits, int64_t l_rs, const float* bias, int32_t* ids, float* weights, int32_t* order,
+                       int32_t* place, int32_t* starts, int32_t* scratch, int tokens, int experts, int k, int sigmoid,
+                       int groups, int top_groups, int renormalize, float scale, void* stream);
+int64_t atma_route_scratch_ints(int tokens, int experts);
+
+/* Row t of q goes to rows place[t * copies + j], j < copies, its scales along. */
+int atma_scatter_rows_fp8(const void* q, int64_t q_rs, const float* scales, int64_t s_bs, const int32_t* place, int copies,
+                          void* to, int64_t to_rs, float* to_scales, int64_t to_bs, int rows, int width, void* stream);
+
+/* out[t] = add[t] (NULL = 0) + sum over j of weights[t][j] y[place[t * copies + j]], in fp32 in this order; dense rows. */
+int atma_combine_experts(const void* y, const int32_t* place, const float* weights, const void* add, void* out, int rows,
+                         int copies, int D, int dtype, void* stream);
+
 /* Status word of this library's tensor-core kernels (see atma_device_status). */
 int atma_decoder_device_status(int* status);
 

@@ -1,0 +1,173 @@
+"""CPU: the oracle of the operators in 8 bits against itself, weights in 8 bits, and what the operators refuse."""
+
+import ctypes
+import math
+import os
+import subprocess
+import tempfile
+import textwrap
+
+import pytest
+import torch
+
+from oracle import fp8 as O
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def test_e4m3_table_and_rounding():
+    v = O.e4m3_values()
+    assert len(v) == 127 and v[-1] == 448 and torch.equal(v.to(torch.float8_e4m3fn).double(), v)
+    x = torch.cat([torch.linspace(-448, 448, 9973, dtype=torch.float64), v, -v])
+    same = O.to_e4m3(x) == x.float().to(torch.float8_e4m3fn).double()
+    assert same.all()
+    b = O.borders()
+    assert torch.equal(O.to_e4m3(b), b.float().to(torch.float8_e4m3fn).double())
+    eps = 2.0 ** -40
+    assert (O.to_e4m3(b * (1 + eps)) > O.to_e4m3(b * (1 - eps))).all()
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (5, 7), (128, 128), (200, 300), (3, 130, 129), (2, 2, 64, 40)])
+def test_weights_in_8_bits(shape):
+    from atma_b200.fp8_ops import Fp8Weight
+    w = torch.randn(*shape, generator=torch.Generator().manual_seed(1))
+    w8 = Fp8Weight.of(w)
+    assert w8.shape == shape and w8.values.data_ptr() % 16 == 0 and (w8.values.stride(-2) % 16 == 0 or shape[:-1] == (1,))
+    s = w8.scales.reshape(-1, *w8.scales.shape[-2:]).double()
+    for m, q, sc in zip(w.reshape(-1, *shape[-2:]).double(), w8.values.reshape(-1, *shape[-2:]), s):
+        for i in range(sc.shape[0]):
+            for j in range(sc.shape[1]):
+                at = (slice(i * 128, (i + 1) * 128), slice(j * 128, (j + 1) * 128))
+                assert sc[i, j] == (m[at].abs().max() / 448).float()
+                assert torch.equal(q[at].double(), O.to_e4m3(m[at] / sc[i, j]))
+    assert (w8.wide() - w).abs().max() <= w.abs().max() * 2.0 ** -4
+    assert torch.equal(Fp8Weight.of(torch.zeros(3, 4)).wide(), torch.zeros(3, 4))
+
+
+def test_rows_and_weights_refuse_what_does_not_fit():
+    from atma_b200.fp8_ops import E4M3, Fp8Rows, Fp8Weight
+    v = torch.zeros(4, 256, dtype=E4M3)
+    Fp8Rows(v, torch.zeros(4, 2))
+    for values, scales in ((v.float(), torch.zeros(4, 2)), (v, torch.zeros(4, 1)), (v, torch.zeros(4, 2, dtype=torch.bfloat16)), (v[0], torch.zeros(2)),
+                           (v, torch.zeros(2, 4))):
+        with pytest.raises(ValueError):
+            Fp8Rows(values, scales)
+    for values, scales in ((v, torch.zeros(4, 2)), (v[0], torch.zeros(2)), (v.float(), torch.zeros(1, 2)), (v[None], torch.zeros(1, 2))):
+        with pytest.raises(ValueError):
+            Fp8Weight(values, scales)
+    r = Fp8Rows(torch.zeros(4, 300, dtype=E4M3)[:, 3:260], torch.zeros(4, 3))            # odd addresses: copied
+    assert r.values.data_ptr() % 16 == 0 and r.values.stride(0) % 16 == 0 and r.scales.stride() == (1, 4)
+    w = Fp8Weight(torch.zeros(2, 300, 4, dtype=E4M3).transpose(1, 2), torch.zeros(2, 1, 3))
+    assert w.values.stride() == (4 * 304, 304, 1)
+    assert Fp8Rows(torch.zeros(1, 5, dtype=E4M3), torch.zeros(1, 1)).shape == (1, 5)
+
+
+def test_operators_refuse_cpu_tensors():
+    from atma_b200 import experts, fp8_ops as f
+    x = torch.zeros(2, 128)
+    r, w = f.Fp8Rows(torch.zeros(2, 128, dtype=f.E4M3), torch.zeros(2, 1)), f.Fp8Weight.of(torch.zeros(3, 128))
+    calls = [lambda: f.quantize_rows(x), lambda: f.residual_norms_fp8(x, None, [x[0]], 1e-6), lambda: f.linear_fp8(r, w), lambda: experts.route_experts(x, 2)]
+    for call in calls:
+        with pytest.raises(RuntimeError):
+            call()
+
+
+@pytest.fixture()
+def anywhere(monkeypatch):
+    """Checks of arguments without a GPU: tensors count as being where they should, and no launch is reached."""
+    from atma_b200 import experts, fp8_ops
+
+    def launch(*a, **kw):
+        raise AssertionError("a refused call came through")
+
+    for m in (fp8_ops, experts):
+        monkeypatch.setattr(m, "_here", lambda *a: None)
+        monkeypatch.setattr(m._lib, "load_decoder", launch)
+    return fp8_ops, experts
+
+
+def test_refused_arguments(anywhere):
+    f, e = anywhere
+    x, y, w = torch.zeros(4, 256), torch.zeros(4, 256, dtype=torch.bfloat16), torch.zeros(256, dtype=torch.bfloat16)
+    r, m = f.Fp8Rows(torch.zeros(4, 256, dtype=f.E4M3), torch.zeros(4, 2)), f.Fp8Weight.of(torch.zeros(8, 256))
+    stack = f.Fp8Weight.of(torch.zeros(6, 2, 32, 256)), f.Fp8Weight.of(torch.zeros(6, 256, 32))
+    routes = e.Routes(torch.zeros(4, 2, dtype=torch.int32), torch.zeros(4, 2), None, None, torch.zeros(7, dtype=torch.int32))
+    z = torch.zeros(4, 12)
+    refused = [
+        lambda: f.quantize_rows(x.half()), lambda: f.quantize_rows(x[0]), lambda: f.quantize_rows(x[:, :0]),
+        lambda: f.residual_norms_fp8(x, y, [], 1e-6), lambda: f.residual_norms_fp8(x, y, [None], 1e-6), lambda: f.residual_norms_fp8(x, y, [w, w, w], 1e-6),
+        lambda: f.residual_norms_fp8(x, x, [w], 1e-6), lambda: f.residual_norms_fp8(x, y[:2], [w], 1e-6), lambda: f.residual_norms_fp8(x, y, [w[:5]], 1e-6),
+        lambda: f.residual_norms_fp8(x.double(), y, [w], 1e-6), lambda: f.residual_norms_fp8(x.t(), y, [w], 1e-6),
+        lambda: f.residual_norms_fp8(x, y, [w], 1e-6, out=y), lambda: f.residual_norms_fp8(x, y, [w.half()], 1e-6),
+        lambda: f.linear_fp8(x, m), lambda: f.linear_fp8(r, x), lambda: f.linear_fp8(r, stack[1]), lambda: f.linear_fp8(r, f.Fp8Weight.of(torch.zeros(8, 128))),
+        lambda: f.linear_fp8(r, m, dtype=torch.float16), lambda: f.linear_fp8(r, m, out=torch.zeros(4, 9)),
+        lambda: f.linear_fp8(r, m, out=torch.zeros(8, 4).t()), lambda: f.linear_fp8(r, m, out=torch.zeros(4, 8, dtype=torch.float64)),
+        lambda: f.linear_fp8(r, m, out=torch.zeros(1, 8).expand(4, 8)),
+        lambda: e.route_experts(z, 0), lambda: e.route_experts(z, 13), lambda: e.route_experts(z, 2, score="relu"), lambda: e.route_experts(z, 2, groups=5),
+        lambda: e.route_experts(z, 2, groups=4, top_groups=5), lambda: e.route_experts(z, 4, groups=4, top_groups=1), lambda: e.route_experts(z, 2, bias=z),
+        lambda: e.route_experts(z.int(), 2), lambda: e.route_experts(z[0], 2), lambda: e.route_experts(torch.zeros(2, 513), 2), lambda: e.route_experts(z[:, :0], 1),
+        lambda: e.route_experts(torch.zeros(2, 200), 65), lambda: e.route_experts(torch.zeros(2, 130), 2, groups=65),
+        lambda: e.expert_mlp(x, *stack, routes), lambda: e.expert_mlp(r[:2], *stack, routes), lambda: e.expert_mlp(r, stack[1], stack[0], routes),
+        lambda: e.expert_mlp(r, *stack, routes, dtype=torch.float16), lambda: e.expert_mlp(r, *stack, routes, add=x),
+        lambda: e.expert_mlp(r, *stack, None),
+    ]
+    for i, call in enumerate(refused):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from atma_b200 import _lib
+    if not os.path.exists(_lib.DECODER_LIB_PATH):
+        from atma_b200.build import build
+        build("decoder")
+    return _lib.load_decoder()
+
+
+def test_the_c_entries_refuse_before_they_launch(lib):
+    from atma_b200 import _lib
+    bad = _lib.ATMA_ERR_INVALID
+    p = ctypes.c_void_p(4096)
+    assert lib.atma_linear_fp8(None, None) == bad
+    good = dict(x=4096, x_rs=256, x_scales=4096, xs_bs=4, w=4096, w_rs=256, w_scales=4096, out=4096, out_rs=64, M=4, N=64, K=250, groups=1, parts=1, dtype=1)
+    for change in (dict(dtype=2), dict(M=-1), dict(N=0), dict(K=0), dict(groups=0), dict(groups=3), dict(parts=3), dict(N=63, parts=2), dict(x=0), dict(w=0),
+                   dict(out=0), dict(x_scales=0), dict(w_scales=0), dict(x=4100), dict(w=4104), dict(x_rs=250), dict(w_rs=240), dict(x_rs=240), dict(out_rs=63),
+                   dict(xs_bs=3), dict(M=1 << 30)):
+        a = _lib.Fp8Args(**{**good, **change})
+        assert lib.atma_linear_fp8(ctypes.byref(a), None) == bad, change
+    assert lib.atma_linear_fp8(ctypes.byref(_lib.Fp8Args(**{**good, "M": 0})), None) == 0
+    assert lib.atma_quantize_rows(p, 8, p, 8, p, 2, 2, 8, 2, None) == bad                # fp16
+    assert lib.atma_quantize_rows(None, 8, p, 16, p, 2, 2, 8, 0, None) == bad
+    assert lib.atma_quantize_rows(p, 8, p, 4, p, 2, 2, 8, 0, None) == bad
+    assert lib.atma_quantize_rows(p, 8, p, 16, p, 1, 2, 8, 0, None) == bad
+    assert lib.atma_quantize_rows(p, 8, p, 16, p, 1, 0, 8, 0, None) == 0
+    route = lambda tokens=4, experts=8, k=2, groups=1, top=1, logits=p, starts=p, l_rs=8: lib.atma_route_experts(
+        logits, l_rs, None, p, p, p, p, starts, p, tokens, experts, k, 0, groups, top, 1, 1.0, None)
+    for kw in (dict(tokens=-1), dict(experts=0), dict(experts=513, l_rs=600), dict(k=0), dict(k=9), dict(groups=3), dict(groups=4, top=5), dict(groups=4, top=0),
+               dict(k=3, groups=4), dict(logits=None), dict(starts=None), dict(l_rs=7), dict(tokens=1 << 30, k=2)):
+        assert route(**kw) == bad, kw
+    assert lib.atma_residual_norms_fp8(p, None, None, p, None, p, None, None, None, None, None, 2, 8, 16, 2, 1e-6, 1.0, 0, None) == bad
+    assert lib.atma_combine_experts(p, p, p, None, None, 2, 2, 8, 0, None) == bad
+    assert lib.atma_scatter_rows_fp8(p, 16, p, 2, p, 0, p, 16, p, 4, 2, 16, None) == bad
+    assert lib.atma_gelu_gate_fp8(p, 15, p, 16, p, 2, 2, 8, None) == bad
+
+
+def test_fp8_args_layout_matches_the_header():
+    from atma_b200 import _lib
+    src = '#include <stdio.h>\n#include "atma_decoder.h"\nint main(void) { printf("%zu\\n", sizeof(atma_fp8_args)); return 0; }\n'
+    with tempfile.TemporaryDirectory() as d:
+        c, exe = os.path.join(d, "s.c"), os.path.join(d, "s")
+        open(c, "w").write(textwrap.dedent(src))
+        subprocess.check_call(["gcc", "-I", os.path.join(ROOT, "include"), c, "-o", exe])
+        assert ctypes.sizeof(_lib.Fp8Args) == int(subprocess.check_output([exe]))
+
+
+def test_routing_oracle_by_hand():
+    ids, w = O.route(torch.tensor([[1.0, 3.0, 2.0, 3.0]]), 2)
+    assert ids == [[1, 3]] and w == [[0.5, 0.5]]
+    z = torch.tensor([[0.0, 5.0, 1.0, 1.0, 4.0, -9.0]])
+    ids, w = O.route(z, 2, "sigmoid", torch.tensor([0, -2.0, 0, 0, 0, 0]), 3, 1, renormalize=False)
+    assert ids == [[2, 3]] and math.isclose(w[0][0], 1 / (1 + math.exp(-1)))
+    assert O.order([[2, 0], [0, 1]], 4) == ([1, 2, 3, 0], [3, 0, 1, 2], [0, 2, 3, 4, 4])

@@ -1,0 +1,216 @@
+"""GPU: routing to experts and their feed-forwards in 8 bits, against fp64 (oracle/fp8.py)."""
+
+import math
+
+import pytest
+import torch
+
+from oracle import fp8 as O
+from tests.test_gpu_fp8 import loud, ops, rand, weight8
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def routing():
+    from atma_b200 import experts
+    return experts
+
+
+def check_order(r):
+    by, place, starts = O.order(r.ids.tolist(), r.experts)
+    assert r.order.tolist() == by and r.place.tolist() == place and r.starts.tolist() == starts
+
+
+ROUTES = [(1, 2, 1, {}), (5, 8, 2, {}), (3, 1, 1, {}), (40, 10, 3, dict(score="sigmoid")), (129, 64, 8, {}), (200, 33, 5, dict(bias=True)),
+          (300, 65, 4, dict(bias=True, score="sigmoid", renormalize=False, scale=2.5)), (150, 256, 8, dict(bias=True, score="sigmoid", groups=8, top_groups=4)),
+          (70, 96, 6, dict(groups=6, top_groups=2)), (64, 40, 7, dict(groups=40, top_groups=9, bias=True)), (50, 512, 16, dict(score="sigmoid", groups=64, top_groups=8)),
+          (37, 300, 64, dict(bias=True)), (6000, 16, 2, dict(bias=True))]
+
+
+@pytest.mark.parametrize("tokens, experts, k, kw", ROUTES)
+def test_route_experts(tokens, experts, k, kw):
+    kw = dict(kw)
+    logits = rand((tokens, experts), tokens, 1.5)
+    bias = rand((experts,), 9, 0.1) if kw.pop("bias", False) else None
+    r = routing().route_experts(logits.cuda(), k, bias=None if bias is None else bias.cuda(), **kw)
+    ids, weights = O.route(logits, k, bias=bias, **kw)
+    assert r.ids.tolist() == ids
+    w = torch.tensor(weights, dtype=torch.float64)
+    # expf, a sum of up to 512 terms over lanes and a quotient, twice: 64 u, and u |z - max| (at most 14 here) of the exponent's argument
+    assert ((r.weights.cpu().double() - w).abs() <= 128 * U * w).all()
+    check_order(r)
+
+
+def test_route_experts_settles_what_fp32_does_not():
+    """Biases that bring every key of a token to within an fp32 rounding of one another: fp64 decides, in groups too."""
+    e = routing()
+    logits = rand((24, 64), 1, 2.0)
+    bias = (0.75 - torch.sigmoid(logits[:1].double())).float()[0]
+    logits[1::2] = logits[0]
+    logits[1::4] += torch.randint(-1, 2, (6, 64), generator=torch.Generator().manual_seed(2)) * 2.0 ** -22
+    for kw in (dict(), dict(groups=8, top_groups=3), dict(groups=16, top_groups=5)):
+        r = e.route_experts(logits.cuda(), 6, score="sigmoid", bias=bias.cuda(), **kw)
+        assert r.ids.tolist() == O.route(logits, 6, "sigmoid", bias, **kw)[0]
+    soft = torch.softmax(logits[0].double(), 0)
+    bias = (0.5 - soft).float()
+    r = e.route_experts(logits.cuda(), 6, bias=bias.cuda())
+    assert r.ids.tolist() == O.route(logits, 6, "softmax", bias)[0]
+
+
+def test_route_experts_equal_keys_take_the_lower_index():
+    e = routing()
+    r = e.route_experts(torch.zeros(3, 40, device="cuda"), 5)
+    assert r.ids.tolist() == [[0, 1, 2, 3, 4]] * 3
+    assert torch.allclose(r.weights, torch.full((3, 5), 0.2, device="cuda"))
+    r = e.route_experts(torch.zeros(2, 40, device="cuda"), 3, score="sigmoid", groups=8, top_groups=2, bias=torch.zeros(40, device="cuda"))
+    assert r.ids.tolist() == [[0, 1, 2]] * 2
+    check_order(r)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("kw", [{}, dict(bias=True), dict(bias=True, groups=4, top_groups=2)])
+def test_route_experts_masked_and_broken_logits(score, kw):
+    kw = dict(kw)
+    x = rand((7, 16), 3)
+    x[0] = -math.inf                                         # nothing left
+    x[1, 3:] = -math.inf
+    x[2, 5] = math.inf
+    x[3] = math.nan
+    x[4, ::2] = math.nan
+    x[5] = torch.finfo(torch.float32).min
+    bias = rand((16,), 4, 0.1) if kw.pop("bias", False) else None
+    r = routing().route_experts(x.cuda(), 4, score=score, bias=None if bias is None else bias.cuda(), **kw)
+    ids, weights = O.route(x, 4, score, bias, **kw)
+    assert r.ids.tolist() == ids
+    w = torch.tensor(weights, dtype=torch.float64)
+    assert ((r.weights.cpu().double() - w).abs() <= 128 * U * w + 1e-37).all()
+    check_order(r)
+
+
+def test_route_experts_with_experts_that_a_bias_rules_out():
+    x, bias = rand((20, 12), 1), torch.zeros(12)
+    bias[2:] = -math.inf
+    r = routing().route_experts(x.cuda(), 3, bias=bias.cuda())
+    assert r.ids.tolist() == O.route(x, 3, bias=bias)[0] and all(set(i[:2]) == {0, 1} for i in r.ids.tolist())
+
+
+def test_route_experts_takes_strided_and_16_bit_logits():
+    x = rand((50, 40), 2)
+    r = routing().route_experts(x.cuda()[:, 4:36], 3)
+    assert r.ids.tolist() == O.route(x[:, 4:36], 3)[0]
+    h = x.bfloat16()
+    assert routing().route_experts(h.cuda(), 3).ids.tolist() == O.route(h.float(), 3)[0]
+    assert routing().route_experts(x.t().contiguous().t().cuda(), 3).ids.tolist() == O.route(x, 3)[0]
+    empty = routing().route_experts(torch.empty(0, 8, device="cuda"), 2)
+    assert empty.ids.shape == (0, 2) and empty.starts.tolist() == [0] * 9
+
+
+def test_route_experts_of_many_tokens_keeps_the_order():
+    """Several chunks, uneven experts: against a stable sort."""
+    x = rand((20000, 24), 5) + torch.linspace(0, 4, 24)
+    r = routing().route_experts(x.cuda(), 3)
+    ids = x.sort(dim=1, descending=True, stable=True).indices[:, :3]
+    assert torch.equal(r.ids.cpu().long(), ids)
+    flat = ids.flatten()
+    assert torch.equal(r.order.cpu().long(), flat.sort(stable=True).indices)
+    assert torch.equal(r.place.cpu().long()[r.order.cpu().long()], torch.arange(60000))
+    assert r.starts.tolist() == [int((flat < e).sum()) for e in range(25)]
+
+
+# tokens, experts, k, width, ff
+MLPS = [(1, 1, 1, 16, 16), (1, 8, 2, 256, 128), (5, 6, 2, 200, 150), (40, 3, 1, 128, 260), (64, 5, 3, 130, 96), (17, 12, 4, 520, 72), (300, 4, 2, 96, 128), (150, 2, 2, 384, 200)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tokens, n, k, width, ff", MLPS)
+def test_expert_mlp(tokens, n, k, width, ff, dtype):
+    e, f = routing(), ops()
+    h = loud(tokens, width, tokens, torch.bfloat16)
+    x = f.quantize_rows(h.cuda())
+    w_in, in_wide = weight8((n, 2, ff, width), 1)
+    w_out, out_wide = weight8((n, width, ff), 2)
+    routes = e.route_experts(rand((tokens, n), 3).cuda(), k, score="sigmoid")
+    add = rand((tokens, width), 4, dtype=dtype)
+    for plus in (None, add):
+        y = e.expert_mlp(x, w_in, w_out, routes, add=None if plus is None else plus.cuda(), dtype=dtype)
+        err = (max(width, ff) + 8) * 2.0 ** -23
+        want, off, most = O.expert_mlp(O.wide_rows(*O.quantize(h.double())), [in_wide[2 * i:2 * i + 2] for i in range(n)], out_wide, routes.ids.tolist(),
+                                       routes.weights.double().tolist(), err)
+        if plus is not None:
+            want, most = want + plus.double(), most + plus.double().abs()
+        half = torch.finfo(dtype).eps / 2                    # an expert's result and the sum; k + 1 additions in fp32
+        off = off + (2 * half + (k + 2) * U) * (most + off)
+        assert y.dtype == dtype and ((y.cpu().double() - want).abs() <= off + 1e-40).all()
+
+
+def test_expert_mlp_where_all_tokens_go_to_one_expert_and_others_have_none():
+    e, f = routing(), ops()
+    logits = torch.zeros(260, 9)
+    logits[:, 4] = 5
+    logits[::3, 7] = 3
+    h = rand((260, 144), 1, dtype=torch.bfloat16)
+    w_in, in_wide = weight8((9, 2, 136, 144), 1)
+    w_out, out_wide = weight8((9, 144, 136), 2)
+    routes = e.route_experts(logits.cuda(), 1)
+    assert routes.starts.tolist() == [0] * 5 + [260] * 5
+    y = e.expert_mlp(f.quantize_rows(h.cuda()), w_in, w_out, routes, dtype=torch.float32)
+    want, off, most = O.expert_mlp(O.wide_rows(*O.quantize(h.double())), [in_wide[2 * i:2 * i + 2] for i in range(9)], out_wide, routes.ids.tolist(),
+                                   routes.weights.double().tolist(), 152 * 2.0 ** -23)
+    assert ((y.cpu().double() - want).abs() <= off + 4 * U * (most + off)).all()
+
+
+def test_expert_mlp_a_broken_token_stays_by_itself_and_the_order_of_tokens_does_not_matter():
+    e, f = routing(), ops()
+    h = rand((90, 256), 1, dtype=torch.bfloat16)
+    logits = rand((90, 6), 2)
+    w_in, _ = weight8((6, 2, 128, 256), 3)
+    w_out, _ = weight8((6, 256, 128), 4)
+
+    def run(h, logits):
+        return e.expert_mlp(f.quantize_rows(h.cuda()), w_in, w_out, e.route_experts(logits.cuda(), 2))
+
+    a = run(h, logits)
+    bad = h.clone()
+    bad[17, 100], bad[40, 3] = math.nan, math.inf
+    b = run(bad, logits)
+    rest = [i for i in range(90) if i not in (17, 40)]
+    assert torch.isnan(b[[17, 40]]).all() and torch.equal(a[rest], b[rest])
+    p = torch.randperm(90, generator=torch.Generator().manual_seed(5))
+    assert torch.equal(run(h[p], logits[p]), a[p.cuda()])
+    assert torch.equal(run(h, logits), a)
+    assert run(h[:0], logits[:0]).shape == (0, 256)
+
+
+def test_norm_routing_and_experts_in_a_graph():
+    """The layer's run of operators, captured: replays on other inputs do what the calls do."""
+    e, f = routing(), ops()
+    w_in, _ = weight8((8, 2, 64, 160), 1)
+    w_out, _ = weight8((8, 160, 64), 2)
+    weight, router = rand((160,), 3, 0.1, torch.bfloat16).cuda(), rand((8, 160), 4, 0.2).cuda()
+    x, y = rand((12, 160), 5).cuda(), rand((12, 160), 6, dtype=torch.bfloat16).cuda()
+
+    def layer(x, y, total):
+        (rows, h), = f.residual_norms_fp8(x, y, [weight], 1e-6, out=total, plain=True)
+        routes = e.route_experts(h.float() @ router.t(), 2)
+        return e.expert_mlp(rows, w_in, w_out, routes, add=y)
+
+    sx, sy, total = x.clone(), y.clone(), torch.empty_like(x)
+    want = layer(x, y, total).clone(), total.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer(sx, sy, total)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer(sx, sy, total)
+    sx.normal_(), sy.normal_()
+    graph.replay()
+    other = layer(sx, sy, torch.empty_like(x))
+    torch.cuda.synchronize()
+    assert torch.equal(out, other)
+    sx.copy_(x), sy.copy_(y)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want[0]) and torch.equal(total, want[1])
