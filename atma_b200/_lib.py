@@ -91,8 +91,9 @@ class Fp8Args(Structure):
     """Mirror of atma_fp8_args (include/atma_decoder.h)."""
     _fields_ = [
         ("x", c_void_p), ("x_rs", c_int64), ("x_scales", c_void_p), ("xs_bs", c_int64),
-        ("w", c_void_p), ("w_rs", c_int64), ("w_scales", c_void_p), ("out", c_void_p), ("out_rs", c_int64), ("starts", c_void_p),
-        ("M", c_int), ("N", c_int), ("K", c_int), ("groups", c_int), ("parts", c_int), ("dtype", c_int),
+        ("w", c_void_p), ("w_rs", c_int64), ("w_scales", c_void_p), ("out", c_void_p), ("out_rs", c_int64),
+        ("out_scales", c_void_p), ("os_bs", c_int64), ("starts", c_void_p),
+        ("M", c_int), ("N", c_int), ("K", c_int), ("groups", c_int), ("form", c_int), ("dtype", c_int),
     ]
 
 
@@ -206,7 +207,6 @@ _DECODER_SIGNATURES = {
     "atma_delta_scan_scratch_bytes": (c_int64, [POINTER(DeltaArgs)]),
     "atma_delta_step": (c_int, [POINTER(DeltaArgs), c_void_p, c_void_p, c_int64, c_float, c_void_p]),
     "atma_quantize_rows": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_void_p]),
-    "atma_gelu_gate_fp8": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_void_p]),
     "atma_residual_norms_fp8": (c_int, [c_void_p] * 11 + [c_int, c_int, c_int64, c_int64, c_float, c_float, c_int, c_void_p]),
     "atma_linear_fp8": (c_int, [POINTER(Fp8Args), c_void_p]),
     "atma_route_experts": (c_int, [c_void_p, c_int64] + [c_void_p] * 7 + [c_int] * 7 + [c_float, c_void_p]),

@@ -1,11 +1,10 @@
-// Row operations around the products in 8 bits: rows to e4m3 with scales, the residual stream's norms with that output, the gelu
-// gate with it, rows copied to the places of their experts and the weighted sum of what comes back.  fp8.cuh says what a block's
+// Row operations around the products in 8 bits: rows to e4m3 with scales, the residual stream's norms with that output,
+// rows copied to the places of their experts and the weighted sum of what comes back.  fp8.cuh says what a block's
 // scale and values are.  A warp owns a block of 128 channels of a row, four of them a lane, so that a block's largest value is a
 // reduction inside of it and nothing is read twice.
 #include "common.cuh"
 #include "early.cuh"
 #include "fp8.cuh"
-#include "gelu.cuh"
 #include "../../include/atma_decoder.h"
 
 namespace atma {
@@ -68,24 +67,6 @@ quantize_rows_kernel(const T* x, int64_t x_rs, uint8_t* q, int64_t q_rs, float* 
 #pragma unroll
   for (int i = 0; i < kQuantBlocks; ++i)
     if (b0 + i < blocks) store_block<kVec>(q + row * q_rs, scales + (b0 + i) * s_bs + row, b0 + i, lane, width, v[i]);
-}
-
-// ---- gelu_tanh(gate) * up to 8 bits -----------------------------------------------------------------------
-// z rows hold [gate: width | up: width] in fp32, as the product leaves them.
-template <bool kVec>
-__global__ void __launch_bounds__(32 * kQuantWarps)
-gelu_gate_fp8_kernel(const float* z, int64_t z_rs, uint8_t* q, int64_t q_rs, float* scales, int64_t s_bs, int64_t pieces, int blocks, int width) {
-  const int64_t piece = (int64_t)blockIdx.x * kQuantWarps + (threadIdx.x >> 5);
-  if (piece >= pieces) return;
-  const int lane = threadIdx.x & 31;
-  const int64_t row = piece / blocks;
-  const int b = (int)(piece - row * blocks);
-  float g[4], u[4];
-  load_block<float, kVec>(z + row * z_rs, b, lane, width, g);
-  load_block<float, kVec>(z + row * z_rs + width, b, lane, width, u);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) g[e] = gelu_tanh_16(g[e]) * u[e];
-  store_block<kVec>(q + row * q_rs, scales + b * s_bs + row, b, lane, width, g);
 }
 
 // ---- the residual stream's norms, in 8 bits ---------------------------------------------------------------
@@ -290,20 +271,6 @@ extern "C" int atma_quantize_rows(const void* x, int64_t x_rs, void* q, int64_t 
     kernel<<<(unsigned)ctas, 32 * kQuantWarps, 0, st>>>((const T*)x, x_rs, (uint8_t*)q, q_rs, scales, s_bs, pieces, per_row, width);
   });
   return launch_status("quantize_rows");
-}
-
-extern "C" int atma_gelu_gate_fp8(const float* z, int64_t z_rs, void* q, int64_t q_rs, float* scales, int64_t s_bs, int rows, int width,
-                                  void* stream) {
-  ATMA_REQUIRE(rows_ok(rows, width) && z_rs >= 2 * (int64_t)width && q_rs >= width && s_bs >= rows, "gelu_gate_fp8: bad shape or strides");
-  if (rows == 0) return ATMA_OK;
-  ATMA_REQUIRE(z != nullptr && q != nullptr && scales != nullptr, "gelu_gate_fp8: null tensors");
-  const int blocks = (width + kFp8Block - 1) / kFp8Block;
-  const int64_t pieces = (int64_t)rows * blocks, ctas = (pieces + kQuantWarps - 1) / kQuantWarps;
-  ATMA_REQUIRE(ctas <= INT32_MAX, "gelu_gate_fp8: too many rows");
-  const bool vec = width % 4 == 0 && z_rs % 4 == 0 && q_rs % 4 == 0 && fits(z, 16) && fits(q, 4);
-  auto* kernel = vec ? gelu_gate_fp8_kernel<true> : gelu_gate_fp8_kernel<false>;
-  kernel<<<(unsigned)ctas, 32 * kQuantWarps, 0, (cudaStream_t)stream>>>(z, z_rs, (uint8_t*)q, q_rs, scales, s_bs, pieces, blocks, width);
-  return launch_status("gelu_gate_fp8");
 }
 
 extern "C" int atma_residual_norms_fp8(const float* x, const void* y, float* x_out, const void* w1, void* q1, float* s1, void* h1,

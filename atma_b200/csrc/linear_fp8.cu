@@ -1,108 +1,648 @@
-// Products of rows and weights in 8 bits: out[m][n] = sum over blocks b of 128 columns of xs[m][b] ws[n / 128][b] sum over the block of
-// x[m][c] w[n][c], for one weight or for every expert's weight and its own rows.
+// Products of rows and weights in 8 bits, out[m][n] = sum over blocks b of 128 columns of xs[m][b] ws[n / 128][b] (x[m], w[n] over b), for
+// one weight or for every expert's weight and its own rows; or gelu_tanh of the first half of a weight's results times the second half,
+// back in 8 bits.
 //
-// 64 x 64 results a CTA, 4 x 4 a thread, fp32 arithmetic.
+// Every block of 128 columns has scales of its own, so that the tensor cores can only sum inside of one: its products (four of 32 columns)
+// go to TMEM, and warps take them from there, times the scales, to sums in registers while the next block's products go to the other
+// half of TMEM.  Sums are fp32 all along.
+//
+// Many rows (linear_fp8_pair_kernel): two SMs share a tile of 256 rows x 256 columns of results (cta_group::2: each holds its 128 rows of x
+// and half of the weight's rows, so that a block is 32 KB a CTA for 512 clocks of products).  Eight warps a CTA keep 128 sums a thread;
+// a block costs them 256 clocks of reading TMEM and as many of fma at most.
+//
+// Few rows (linear_fp8_rows_kernel): the weight's rows are the tensor core's rows, 128 a tile, and the tokens its columns, 16 to 64, so
+// that a stage is all weight.  Bound by reading that: two CTAs an SM with 100 KB of copies in flight each.  Where a dense product has too few
+// tiles for that, a cluster shares one: every CTA takes its part of the columns, and each then adds up what all of them have for
+// some of the tokens, from their shared memory and in their order.
+//
+// Every mbarrier wait is bounded; on expiry the CTAs free their TMEM, return and leave a status word for the host.
 #include "common.cuh"
+#include "early.cuh"
+#include "f32x2.cuh"
 #include "fp8.cuh"
+#include "gelu.cuh"
+#include "linear_fp8.cuh"
+#include "sm100_pair.cuh"
 #include "../../include/atma_decoder.h"
 
 namespace atma {
 
 namespace {
 
-constexpr int kTile = 64, kCols = 32;
+using namespace sm100;
 
-__device__ __forceinline__ float wide(uint8_t v) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(v, __NV_E4M3)));
+constexpr int kBM = 128, kBK = 128;                         // rows of a plane, columns (= bytes) of a stage
+constexpr int kPlane = kBM * kBK;
+constexpr int kMaxGroups = 512;
+
+__device__ int g_linear_fp8_status = 0;
+
+struct Args {
+  const float *x_scales, *w_scales;
+  void* out;
+  float* out_scales;
+  const int32_t* starts;
+  int64_t xs_bs, out_rs, os_bs;
+  int M, width, K, groups, nb, kb;          // width: columns of results (of one half in the gated form); nb, kb: blocks of width and of K
+  bool vec;                                 // rows of out start on 16-byte boundaries
+};
+
+// Tiles of every group's rows, `tall` rows each: s_first[g] of them in front of group g's.  Called by a whole warp.
+__device__ __forceinline__ void count_tiles(int* s_first, const Args& a, int tall) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int g0 = 0; g0 < a.groups; g0 += 32) {
+    const int g = g0 + lane;
+    int n = 0;
+    if (g < a.groups) {
+      const int lo = a.starts == nullptr ? 0 : min(max(a.starts[g], 0), a.M), hi = a.starts == nullptr ? a.M : min(max(a.starts[g + 1], 0), a.M);
+      n = hi > lo ? (hi - lo + tall - 1) / tall : 0;
+    }
+    int in = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, in, o);
+      if (lane >= o) in += t;
+    }
+    if (g < a.groups) s_first[g] = before + in - n;
+    before += __shfl_sync(0xffffffffu, in, 31);
+  }
+  if (lane == 0) s_first[a.groups] = before;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256)
-linear_fp8_kernel(const atma_fp8_args a) {
-  __shared__ float s_x[kCols][kTile + 1], s_w[kCols][kTile + 1];
-  __shared__ int s_place[3];
-  const int tid = threadIdx.x;
-  if (tid == 0) {                           // which group's rows, and which of them
-    int tile = blockIdx.x, g = 0, lo = 0, hi = a.starts == nullptr ? a.M : 0;
-    s_place[0] = -1;
-    for (; g < a.groups; ++g) {
-      if (a.starts != nullptr) { lo = a.starts[g]; hi = a.starts[g + 1]; }
-      const int n = (hi - lo + kTile - 1) / kTile;
-      if (tile < n) { s_place[0] = g; s_place[1] = lo + tile * kTile; s_place[2] = hi; break; }
-      tile -= n;
-    }
+struct Place { int group, m0, m1, n0; };    // rows m0 .. of group, whose rows end at m1; columns n0 ..
+
+// Tile `tile` of the groups' n_tiles x (tiles of rows), `beside` tiles of rows beside one another.
+__device__ __forceinline__ Place place_of(int tile, const int* s_first, const Args& a, int tall, int wide, int n_tiles, int beside) {
+  int lo = 0, hi = a.groups;                // the last group with s_first * n_tiles <= tile (empty ones are passed over)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (s_first[mid] * n_tiles <= tile) lo = mid; else hi = mid;
   }
+  const int m_tiles = s_first[lo + 1] - s_first[lo], at = tile - s_first[lo] * n_tiles;
+  const int band = at / (beside * n_tiles), in = at - band * beside * n_tiles, high = min(beside, m_tiles - band * beside);
+  Place p;
+  p.group = lo;
+  const int first = a.starts == nullptr ? 0 : min(max(a.starts[lo], 0), a.M);
+  p.m1 = a.starts == nullptr ? a.M : min(max(a.starts[lo + 1], 0), a.M);
+  p.m0 = first + (band * beside + in % high) * tall;
+  p.n0 = in / high * wide;
+  return p;
+}
+
+// A barrier of kCount threads at which all of them learn whether one has given up: they leave their loops together.
+template <int kCount>
+__device__ __forceinline__ bool any_gave_up(bool mine) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "barrier.cta.red.or.pred p, 1, %2, q;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(any) : "r"((uint32_t)mine), "n"(kCount) : "memory");
+  return any != 0;
+}
+
+// ---- many rows -------------------------------------------------------------------------------------------
+constexpr int kStages = 5, kStageBytes = 2 * kPlane;
+constexpr int kSumWarps = 8, kPairThreads = 128 + 32 * kSumWarps;
+constexpr int kStaging = 32 * 128;                          // bytes of a warp's 32 rows x 128 bytes of results
+constexpr int kPairSmem = kStages * kStageBytes + kSumWarps * kStaging + 1024;
+constexpr int kBeside = 8;
+
+// 32 sums of a thread's row += scale * the products in r.
+__device__ __forceinline__ void add_scaled(uint64_t* sum, uint32_t* r, float scale) {
+  const uint64_t s2 = pack2(scale, scale);
+#pragma unroll
+  for (int i = 0; i < 32; ++i) reg_fence(r[i]);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) sum[i] = fma2(pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), s2, sum[i]);
+}
+
+template <typename T, bool kGated>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ Args a) {
+  constexpr int kTileN = kGated ? 128 : 256;                // columns of results of a tile
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];      // full and acc_empty: the first CTA's are used
+  __shared__ uint32_t s_tmem;
+  __shared__ volatile int s_abort_v;
+  __shared__ int s_first[kMaxGroups + 1];
+  __shared__ float s_most[kGated ? 2 : 1][2][kGated ? 128 : 1];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint32_t rank;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  if (warp == 2) count_tiles(s_first, a, 2 * kBM);
+  if (tid == 32) {
+    for (int i = 0; i < kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 2 * kSumWarps); }
+    s_abort_v = 0;
+    fence_barrier_init();
+  }
+  tc_fence_before();
   __syncthreads();
-  if (s_place[0] < 0) return;
-  const int g = s_place[0], m0 = s_place[1], m1 = s_place[2], n0 = blockIdx.y * kTile;
-  const int kb = (a.K + kFp8Block - 1) / kFp8Block, width = a.N / a.parts, nb = (width + kFp8Block - 1) / kFp8Block;
-  const uint8_t *x = (const uint8_t*)a.x, *w = (const uint8_t*)a.w + (int64_t)g * a.N * a.w_rs;
-  const float* ws = a.w_scales + (int64_t)g * a.parts * nb * kb;
-  const int ty = tid >> 4, tx = tid & 15;
-  float sum[4][4] = {}, part[4][4];
-  for (int c0 = 0; c0 < a.K; c0 += kCols) {
-    if (c0 % kFp8Block == 0)
+  cluster_sync();                           // the neighbour's barriers are there
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  const int n_tiles = (a.width + kTileN - 1) / kTileN, tiles = s_first[a.groups] * n_tiles;
+  volatile int* abort = &s_abort_v;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 0) {
+      if (elect_one()) {
+        uint32_t n = 0;                     // blocks so far, over all tiles
+        bool ok = true;
+        for (int tile = pair; tile < tiles && ok; tile += pairs) {
+          const Place p = place_of(tile, s_first, a, 2 * kBM, kTileN, n_tiles, kBeside);
+          const int xr = p.m0 + (int)rank * kBM;
+          const int wr = kGated ? (2 * p.group + (int)rank) * a.width + p.n0 : p.group * a.width + p.n0 + (int)rank * kBM;
+          for (int it = 0; it < a.kb; ++it, ++n) {
+            const uint32_t st = n % kStages;
+            if (n >= kStages && !(ok = mbar_wait(&empty[st], (n / kStages - 1) & 1, abort))) break;
+            uint8_t* to = smem + st * kStageBytes;
+            if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * kStageBytes);
+            const uint32_t bar = in_first(smem_u32(&full[st]));
+            tma_load_pair(to, &tm_x, bar, it * kBK, xr);
+            tma_load_pair(to + kPlane, &tm_w, bar, it * kBK, wr);
+          }
+        }
+        // whatever the others do, the CTA does not end before its copies have landed and the products that read them are done
+        volatile int alone = 0;
+        for (uint32_t i = n > kStages ? n - kStages : 0; i < n; ++i)
+          if (!mbar_wait(&empty[i % kStages], (i / kStages) & 1, &alone)) { *abort = 1; break; }
+      }
+    } else if (warp == 1) {
+      if (rank == 0 && elect_one()) {
+        constexpr uint32_t idesc = make_idesc(2 * kBM, 2 * kBM, 0, 0, 0);
+        uint32_t n = 0;
+        bool ok = true;
+        for (int tile = pair; tile < tiles && ok; tile += pairs) {
+          for (int it = 0; it < a.kb; ++it, ++n) {
+            const uint32_t st = n % kStages, buf = n & 1;
+            if (n >= 2 && !(ok = mbar_wait(&acc_empty[buf], (n / 2 - 1) & 1, abort))) break;
+            if (!(ok = mbar_wait(&full[st], (n / kStages) & 1, abort))) break;
+            tc_fence_after();
+            const uint32_t at = smem_u32(smem + st * kStageBytes), d = tmem + buf * 2 * kBM;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) part[i][j] = 0.f;
-    for (int i = tid; i < kTile * kCols; i += 256) {
-      const int r = i / kCols, c = i % kCols;
-      s_x[c][r] = m0 + r < m1 && c0 + c < a.K ? wide(x[(int64_t)(m0 + r) * a.x_rs + c0 + c]) : 0.f;
-      s_w[c][r] = n0 + r < a.N && c0 + c < a.K ? wide(w[(int64_t)(n0 + r) * a.w_rs + c0 + c]) : 0.f;
+            for (int k = 0; k < kBK / 32; ++k)
+              mma_pair_8bit(d, make_sdesc_sw128(at + 32 * k, 16, 1024), make_sdesc_sw128(at + kPlane + 32 * k, 16, 1024), idesc, k > 0);
+            commit_pair(&empty[st]);
+            commit_pair(&acc_full[buf]);
+          }
+        }
+      }
     }
-    __syncthreads();
-    for (int c = 0; c < kCols; ++c)
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int w = warp - 4, quarter = warp & 3, side = w >> 2;
+    uint8_t* s = smem + kStages * kStageBytes + w * kStaging;
+    uint32_t n = 0, turn = 0;
+    bool ok = true;
+    for (int tile = pair; tile < tiles && ok; tile += pairs, turn ^= 1) {
+      const Place p = place_of(tile, s_first, a, 2 * kBM, kTileN, n_tiles, kBeside);
+      const int row0 = p.m0 + (int)rank * kBM + 32 * quarter, row = row0 + lane;
+      // gated: 64 columns of either half a thread, the halves 128 columns of TMEM apart; else 128 columns of results
+      const int c0 = kGated ? 64 * side : 128 * side, behind = kGated ? 128 : 64;
+      const float* xs = a.x_scales + min(row, a.M - 1);
+      const float* ws = a.w_scales + (kGated ? ((int64_t)(2 * p.group) * a.nb + p.n0 / 128) : ((int64_t)p.group * a.nb + min(p.n0 / 128 + side, a.nb - 1))) * a.kb;
+      const float* us = ws + (kGated ? (int64_t)a.nb * a.kb : 0);
+      uint64_t sum[64];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 64; ++i) sum[i] = 0;
+      float fx = xs[0], fw = ws[0], fu = us[0];
+      for (int it = 0; it < a.kb; ++it, ++n) {
+        const uint32_t buf = n & 1, at = tmem + (uint32_t(32 * quarter) << 16) + buf * 2 * kBM + c0;
+        const float sw = fx * fw, su = fx * fu;
+        if (it + 1 < a.kb) { fx = xs[(int64_t)(it + 1) * a.xs_bs]; fw = ws[it + 1]; fu = us[it + 1]; }
+        if (!(ok = mbar_wait_warp(&acc_full[buf], (n / 2) & 1, abort))) break;
+        tc_fence_after();
+        uint32_t r0[32], r1[32];
+        tmem_ld32_nowait(at, r0);
+        tmem_ld_wait();
+        tmem_ld32_nowait(at + 32, r1);
+        add_scaled(sum, r0, sw);
+        tmem_ld_wait();
+        tmem_ld32_nowait(at + behind, r0);
+        add_scaled(sum + 16, r1, sw);
+        tmem_ld_wait();
+        tmem_ld32_nowait(at + behind + 32, r1);
+        add_scaled(sum + 32, r0, su);
+        tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 4; ++j) part[i][j] = fmaf(s_x[c][ty + 16 * i], s_w[c][tx + 16 * j], part[i][j]);
-    __syncthreads();
-    if ((c0 + kCols) % kFp8Block == 0 || c0 + kCols >= a.K) {
-      const int b = c0 / kFp8Block;
+        for (int i = 0; i < 32; ++i) reg_fence(r1[i]);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_cluster(in_first(smem_u32(&acc_empty[buf])));
+        add_scaled(sum + 48, r1, su);
+      }
+      if constexpr (!kGated)
+        if (!ok) break;
+      if constexpr (kGated) {
+        const int f0 = p.n0 + 64 * side;
+        float v[64], most = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int m = m0 + ty + 16 * i;
-        const float xs = m < m1 ? a.x_scales[(int64_t)b * a.xs_bs + m] : 0.f;
+        for (int i = 0; i < 32; ++i) {
+          const float2 g = unpack2(sum[i]), u = unpack2(sum[32 + i]);
+          v[2 * i] = f0 + 2 * i < a.width ? gelu_tanh_16(g.x) * u.x : 0.f;
+          v[2 * i + 1] = f0 + 2 * i + 1 < a.width ? gelu_tanh_16(g.y) * u.y : 0.f;
+          most = max_nan(most, max_nan(fabsf(v[2 * i]), fabsf(v[2 * i + 1])));
+        }
+        // a block's 128 columns are two warps': its largest value through shared memory, in turns of two
+        s_most[turn][side][32 * quarter + lane] = most;
+        if (any_gave_up<256>(!ok || *abort)) break;
+        const float scale = fp8_scale(max_nan(s_most[turn][0][32 * quarter + lane], s_most[turn][1][32 * quarter + lane]));
+        if (row < p.m1) {
+          if (side == 0) a.out_scales[(int64_t)(p.n0 / 128) * a.os_bs + row] = scale;
+          uint8_t* to = static_cast<uint8_t*>(a.out) + (int64_t)row * a.out_rs + f0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int n = n0 + tx + 16 * j;
-          if (n < a.N) sum[i][j] = fmaf(part[i][j], xs * ws[((int64_t)(n / width) * nb + n % width / kFp8Block) * kb + b], sum[i][j]);
+          for (int i = 0; i < 64; i += 16) {
+            uint32_t q[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float four[4] = {v[i + 4 * j], v[i + 4 * j + 1], v[i + 4 * j + 2], v[i + 4 * j + 3]};
+              q[j] = fp8_four(four, scale);
+            }
+            if (f0 + i + 16 <= a.width) *reinterpret_cast<uint4*>(to + i) = make_uint4(q[0], q[1], q[2], q[3]);
+            else
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                if (f0 + i + j < a.width) to[i + j] = (uint8_t)(q[j >> 2] >> 8 * (j & 3));
+          }
+        }
+      } else {
+        constexpr int kCols = 128 / sizeof(T), kPer = 16 / sizeof(T);              // columns of a chunk of 128 bytes, of a piece of 16
+        T* out = static_cast<T*>(a.out);
+#pragma unroll
+        for (int chunk = 0; chunk < 128 / kCols; ++chunk) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            alignas(16) T o[kPer];
+#pragma unroll
+            for (int j = 0; j < kPer; j += 2) {
+              const float2 f = unpack2(sum[(chunk * kCols + q * kPer + j) / 2]);
+              o[j] = from_f32<T>(f.x);
+              o[j + 1] = from_f32<T>(f.y);
+            }
+            *reinterpret_cast<uint4*>(s + lane * 128 + ((q ^ (lane & 7)) << 4)) = *reinterpret_cast<const uint4*>(o);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {     // four rows at a time, 128 bytes each
+            const int r = 4 * i + (lane >> 3), q = lane & 7, col = p.n0 + c0 + chunk * kCols + q * kPer;
+            const uint4 v = *reinterpret_cast<const uint4*>(s + r * 128 + ((q ^ (r & 7)) << 4));
+            if (row0 + r >= p.m1) continue;
+            T* to = out + (int64_t)(row0 + r) * a.out_rs + col;
+            if (a.vec && col + kPer <= a.width) *reinterpret_cast<uint4*>(to) = v;
+            else {
+              const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+              for (int j = 0; j < kPer; ++j)
+                if (col + j < a.width) to[j] = e[j];
+            }
+          }
+          __syncwarp();
         }
       }
     }
   }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();                           // nobody signals a CTA that is gone
+  tc_fence_after();
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if (tid == 0 && s_abort_v) atomicExch(&g_linear_fp8_status, 1);
+}
+
+// ---- few rows --------------------------------------------------------------------------------------------
+constexpr int kRowsThreads = 192;
+
+template <int NT, bool kGated>
+struct Few {
+  static constexpr int kHalves = kGated ? 2 : 1;
+  static constexpr int kStageBytes = kHalves * kPlane + NT * kBK;
+  static constexpr int kCtas = kHalves * NT >= 128 ? 1 : 2; // of an SM: with 128 sums and as many products a thread there is one
+  static constexpr int kStages = (kCtas == 1 ? 208 : 104) * 1024 / kStageBytes;
+  static constexpr int kBufs = kHalves * NT >= 128 ? 2 : 4, kColumns = kBufs * kHalves * NT;
+  static constexpr int kSmem = kStages * kStageBytes + 1024;
+  static_assert(kColumns <= 256 && kColumns >= 32 && (kColumns & (kColumns - 1)) == 0, "two CTAs share an SM's TMEM");
+  static_assert(kHalves * NT * 128 * 4 <= kStages * kStageBytes, "a cluster's sums lie where the copies were");
+};
+
+template <typename T, int NT, bool kGated>
+__global__ void __launch_bounds__(kRowsThreads, Few<NT, kGated>::kCtas)
+linear_fp8_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ Args a) {
+  using F = Few<NT, kGated>;
+  constexpr int kHalves = F::kHalves;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full[F::kStages], empty[F::kStages], acc_full[F::kBufs], acc_empty[F::kBufs];
+  __shared__ uint32_t s_tmem;
+  __shared__ volatile int s_abort_v;
+  __shared__ int s_first[kMaxGroups + 1];
+  __shared__ __align__(16) float s_scale[4][2][kHalves][NT];
+  __shared__ float s_most[kGated ? 4 : 1][kGated ? NT : 1];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint32_t rank, ranks;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+  const int worker = blockIdx.x / ranks, workers = gridDim.x / ranks;
+
+  early_start();
+  if (warp == 0) tmem_alloc(&s_tmem, F::kColumns);
+  if (warp == 2) count_tiles(s_first, a, NT);
+  if (tid == 32) {
+    for (int i = 0; i < F::kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+    for (int i = 0; i < F::kBufs; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 4); }
+    s_abort_v = 0;
+    fence_barrier_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  const int n_tiles = (a.width + kBM - 1) / kBM, tiles = s_first[a.groups] * n_tiles;
+  // a cluster's CTAs share the columns of its one tile
+  const int k0 = (int)((int64_t)a.kb * rank / ranks), k1 = (int)((int64_t)a.kb * (rank + 1) / ranks);
+  volatile int* abort = &s_abort_v;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      uint32_t n = 0;
+      bool ok = true;
+      for (int tile = worker; tile < tiles && ok; tile += workers) {
+        const Place p = place_of(tile, s_first, a, NT, kBM, n_tiles, 1 << 20);
+        for (int it = k0; it < k1; ++it, ++n) {
+          const uint32_t st = n % F::kStages;
+          if (n >= F::kStages && !(ok = mbar_wait(&empty[st], (n / F::kStages - 1) & 1, abort))) break;
+          uint8_t* to = smem + st * F::kStageBytes;
+          mbar_arrive_expect_tx(&full[st], F::kStageBytes);
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-      if (m < m1 && n < a.N) ((T*)a.out)[(int64_t)m * a.out_rs + n] = from_f32<T>(sum[i][j]);
+          for (int h = 0; h < kHalves; ++h)
+            tma_load_4d(to + h * kPlane, &tm_w, &full[st], it * kBK, (kHalves * p.group + h) * a.width + p.n0, 0, 0);
+          tma_load_4d(to + kHalves * kPlane, &tm_x, &full[st], it * kBK, p.m0, 0, 0);
+        }
+      }
+      volatile int alone = 0;               // see above
+      for (uint32_t i = n > F::kStages ? n - F::kStages : 0; i < n; ++i)
+        if (!mbar_wait(&empty[i % F::kStages], (i / F::kStages) & 1, &alone)) { *abort = 1; break; }
     }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      constexpr uint32_t idesc = make_idesc(kBM, NT, 0, 0, 0);
+      uint32_t n = 0;
+      bool ok = true;
+      for (int tile = worker; tile < tiles && ok; tile += workers) {
+        for (int it = k0; it < k1; ++it, ++n) {
+          const uint32_t st = n % F::kStages, buf = n % F::kBufs;
+          if (n >= F::kBufs && !(ok = mbar_wait(&acc_empty[buf], (n / F::kBufs - 1) & 1, abort))) break;
+          if (!(ok = mbar_wait(&full[st], (n / F::kStages) & 1, abort))) break;
+          tc_fence_after();
+          const uint32_t at = smem_u32(smem + st * F::kStageBytes), d = tmem + buf * kHalves * NT;
+#pragma unroll
+          for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+            for (int k = 0; k < kBK / 32; ++k)
+              mma_8bit(d + h * NT, make_sdesc_sw128(at + h * kPlane + 32 * k, 16, 1024), make_sdesc_sw128(at + kHalves * kPlane + 32 * k, 16, 1024), idesc, k > 0);
+          tc_commit(&empty[st]);
+          tc_commit(&acc_full[buf]);
+        }
+      }
+    }
+  } else {
+    const int quarter = warp & 3, feature = 32 * quarter + lane;         // of the tile's 128
+    uint32_t n = 0;
+    bool ok = true;
+    for (int tile = worker; tile < tiles && ok; tile += workers) {
+      const Place p = place_of(tile, s_first, a, NT, kBM, n_tiles, 1 << 20);
+      const int rows = min(NT, p.m1 - p.m0), col = p.n0 + feature;
+      const float* ws = a.w_scales + ((int64_t)kHalves * p.group * a.nb + p.n0 / 128) * a.kb;
+      const float* us = ws + (kGated ? (int64_t)a.nb * a.kb : 0);
+      uint64_t sum[kHalves][NT / 2];
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+        for (int i = 0; i < NT / 2; ++i) sum[h][i] = 0;
+      // lane l brings the scales of tokens l and l + 32, one block ahead
+      constexpr int kOwn = (NT + 31) / 32;
+      float fx[kOwn], fw, fu;
+      auto bring = [&](int it) {
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) fx[i] = lane + 32 * i < rows ? a.x_scales[it * a.xs_bs + p.m0 + lane + 32 * i] : 0.f;
+        fw = ws[it];
+        fu = us[it];
+      };
+      bring(k0);
+      for (int it = k0; it < k1; ++it, ++n) {
+        const uint32_t buf = n % F::kBufs;
+        float(&sc)[kHalves][NT] = s_scale[quarter][n & 1];
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i)
+          if (lane + 32 * i < NT) {
+            sc[0][lane + 32 * i] = fx[i] * fw;
+            if constexpr (kGated) sc[kHalves - 1][lane + 32 * i] = fx[i] * fu;
+          }
+        __syncwarp();
+        if (it + 1 < k1) bring(it + 1);
+        if (!(ok = mbar_wait_warp(&acc_full[buf], (n / F::kBufs) & 1, abort))) break;
+        tc_fence_after();
+        const uint32_t at = tmem + (uint32_t(32 * quarter) << 16) + buf * kHalves * NT;
+        uint32_t r[kHalves][NT];
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+          for (int c = 0; c < NT; c += 16) tmem_ld16_nowait(at + h * NT + c, &r[h][c]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+          for (int c = 0; c < NT; ++c) reg_fence(r[h][c]);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[buf]);
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+          for (int c = 0; c < NT; c += 4) {
+            const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(&sc[h][c]);
+            sum[h][c / 2] = fma2(pack2(__uint_as_float(r[h][c]), __uint_as_float(r[h][c + 1])), f.x, sum[h][c / 2]);
+            sum[h][c / 2 + 1] = fma2(pack2(__uint_as_float(r[h][c + 2]), __uint_as_float(r[h][c + 3])), f.y, sum[h][c / 2 + 1]);
+          }
+      }
+      if (!kGated || ranks > 1)
+        if (!ok) break;
+      if (ranks > 1) {                      // what this CTA has, to where its copies were: all of them have been read
+        float* part = reinterpret_cast<float*>(smem);
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+          for (int c = 0; c < NT; c += 2) {
+            const float2 f = unpack2(sum[h][c / 2]);
+            part[(h * NT + c) * 128 + feature] = f.x;
+            part[(h * NT + c + 1) * 128 + feature] = f.y;
+          }
+        break;                              // a cluster has one tile
+      }
+      if constexpr (kGated) {
+        float v[NT];
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+          const float2 g = unpack2(sum[0][c / 2]), u = unpack2(sum[kHalves - 1][c / 2]);
+          v[c] = col < a.width ? gelu_tanh_16(c & 1 ? g.y : g.x) * (c & 1 ? u.y : u.x) : 0.f;
+          if (c < rows) {
+            const float most = warp_max_nan(fabsf(v[c]));
+            if (lane == 0) s_most[quarter][c] = most;
+          }
+        }
+        if (any_gave_up<128>(!ok || *abort)) break;
+#pragma unroll
+        for (int c = 0; c < NT; ++c)
+          if (c < rows) {
+            const float scale = fp8_scale(max_nan(max_nan(s_most[0][c], s_most[1][c]), max_nan(s_most[2][c], s_most[3][c])));
+            if (feature == 0) a.out_scales[(int64_t)(p.n0 / 128) * a.os_bs + p.m0 + c] = scale;
+            if (col < a.width) static_cast<uint8_t*>(a.out)[(int64_t)(p.m0 + c) * a.out_rs + col] = fp8_one(v[c], scale);
+          }
+        asm volatile("bar.sync 1, 128;" ::: "memory");       // s_most is read
+      } else if (col < a.width) {
+        T* out = static_cast<T*>(a.out) + (int64_t)p.m0 * a.out_rs + col;
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+          const float2 f = unpack2(sum[0][c / 2]);
+          if (c < rows) out[c * a.out_rs] = from_f32<T>(c & 1 ? f.y : f.x);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  if (ranks > 1) {                          // the same for all of the cluster
+    __syncthreads();
+    cluster_sync();
+    if (warp >= 2 && worker < tiles) {
+      const Place p = place_of(worker, s_first, a, NT, kBM, n_tiles, 1 << 20);
+      const int feature = 32 * (warp & 3) + lane, rows = min(NT, p.m1 - p.m0), col = p.n0 + feature;
+      for (int c = rank; c < rows; c += ranks) {
+        float v[kHalves] = {};
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+          const uint32_t mine = smem_u32(smem) + ((h * NT + c) * 128 + feature) * 4;
+          for (uint32_t o = 0; o < ranks; ++o) {
+            uint32_t there;
+            float f;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(mine), "r"(o));
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(there) : "memory");
+            v[h] += f;
+          }
+        }
+        if constexpr (kGated) {
+          v[0] = col < a.width ? gelu_tanh_16(v[0]) * v[kHalves - 1] : 0.f;
+          const float most = warp_max_nan(fabsf(v[0]));
+          if (lane == 0) s_most[warp & 3][c] = most;
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+          const float scale = fp8_scale(max_nan(max_nan(s_most[0][c], s_most[1][c]), max_nan(s_most[2][c], s_most[3][c])));
+          if (feature == 0) a.out_scales[(int64_t)(p.n0 / 128) * a.os_bs + p.m0 + c] = scale;
+          if (col < a.width) static_cast<uint8_t*>(a.out)[(int64_t)(p.m0 + c) * a.out_rs + col] = fp8_one(v[0], scale);
+        } else if (col < a.width) {
+          static_cast<T*>(a.out)[(int64_t)(p.m0 + c) * a.out_rs + col] = from_f32<T>(v[0]);
+        }
+      }
+    }
+    cluster_sync();                         // nobody reads a CTA that is gone
+  }
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) tmem_dealloc(tmem, F::kColumns);
+  if (tid == 0 && s_abort_v) atomicExch(&g_linear_fp8_status, 1);
+}
+
+template <typename T, bool kGated>
+int launch_pair(const CUtensorMap& x, const CUtensorMap& w, const Args& a, cudaStream_t st) {
+  auto kern = linear_fp8_pair_kernel<T, kGated>;
+  ATMA_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+  const int64_t n_tiles = (a.width + (kGated ? 127 : 255)) / (kGated ? 128 : 256);
+  const int64_t tiles = (a.M / (2 * kBM) + (a.groups < a.M ? a.groups : a.M)) * n_tiles;       // at most
+  ATMA_REQUIRE(tiles < INT32_MAX / 2, "linear_fp8: too many tiles");
+  const int pairs = sm_count_of_current_device() / 2;
+  kern<<<2 * (unsigned)(tiles < pairs ? tiles : pairs), kPairThreads, kPairSmem, st>>>(x, w, a);
+  return launch_status("linear_fp8 (many rows)");
+}
+
+template <typename T, int NT, bool kGated>
+int launch_rows(const CUtensorMap& x, const CUtensorMap& w, const Args& a, cudaStream_t st) {
+  using F = Few<NT, kGated>;
+  auto kern = linear_fp8_rows_kernel<T, NT, kGated>;
+  ATMA_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem));
+  const int64_t n_tiles = (a.width + kBM - 1) / kBM, slots = F::kCtas * (int64_t)sm_count_of_current_device();
+  const int64_t tiles = (a.starts == nullptr ? (a.M + NT - 1) / NT : a.M / NT + (a.groups < a.M ? a.groups : a.M)) * n_tiles;
+  ATMA_REQUIRE(tiles < INT32_MAX / 2, "linear_fp8: too many tiles");
+  int ranks = 1;                            // CTAs that share a tile, four blocks each at least
+  if (a.starts == nullptr)
+    while (ranks < 8 && 2 * ranks * tiles <= slots && 4 * 2 * ranks <= a.kb) ranks *= 2;
+  cudaLaunchAttribute attrs[1];
+  attrs[0].id = cudaLaunchAttributeClusterDimension;
+  attrs[0].val.clusterDim.x = ranks; attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3((unsigned)(tiles < slots / ranks ? tiles : slots / ranks) * ranks); c.blockDim = dim3(kRowsThreads);
+  c.dynamicSmemBytes = F::kSmem; c.stream = st; c.attrs = attrs; c.numAttrs = 1;
+  ATMA_CUDA_OK(cudaLaunchKernelEx(&c, kern, x, w, a));
+  return launch_status("linear_fp8 (few rows)");
+}
+
+template <typename T, bool kGated>
+int launch(const atma_fp8_args& f, const Args& a, cudaStream_t st) {
+  // rows of a group, if all have as many
+  const int each = (a.M + a.groups - 1) / a.groups, nt = each <= 16 ? 16 : each <= 32 ? 32 : each <= 128 ? 64 : 0;
+  CUtensorMap x, w;
+  int rc = make_tmap_8bit_rows(&x, f.x, a.M, f.x_rs, a.K, nt > 0 ? nt : kBM);
+  if (rc == ATMA_OK) rc = make_tmap_8bit_rows(&w, f.w, (uint64_t)a.groups * f.N, f.w_rs, a.K, kBM);
+  if (rc != ATMA_OK) return rc;
+  if (nt == 16) return launch_rows<T, 16, kGated>(x, w, a, st);
+  if (nt == 32) return launch_rows<T, 32, kGated>(x, w, a, st);
+  if (nt == 64) return launch_rows<T, 64, kGated>(x, w, a, st);
+  return launch_pair<T, kGated>(x, w, a, st);
 }
 
 }  // namespace
+
+int linear_fp8_status_fetch_and_clear(int* out) {
+  int v = 0, zero = 0;
+  ATMA_CUDA_OK(cudaMemcpyFromSymbol(&v, g_linear_fp8_status, sizeof(int)));
+  if (v != 0) ATMA_CUDA_OK(cudaMemcpyToSymbol(g_linear_fp8_status, &zero, sizeof(int)));
+  *out = v;
+  return ATMA_OK;
+}
+
 }  // namespace atma
 
 using namespace atma;
 
 extern "C" int atma_linear_fp8(const atma_fp8_args* args, void* stream) {
   ATMA_REQUIRE(args != nullptr, "linear_fp8: null args");
-  const atma_fp8_args& a = *args;
-  ATMA_REQUIRE(a.dtype == ATMA_F32 || a.dtype == ATMA_BF16, "linear_fp8: unsupported dtype %d", a.dtype);
-  ATMA_REQUIRE(a.M >= 0 && a.M <= (1 << 28) && a.N > 0 && a.N <= (1 << 24) && a.K > 0 && a.K <= (1 << 24), "linear_fp8: bad shape (%d, %d, %d)", a.M, a.N, a.K);
-  ATMA_REQUIRE(a.groups > 0 && a.groups <= 65536 && (a.starts != nullptr || a.groups == 1), "linear_fp8: %d groups without their rows", a.groups);
-  ATMA_REQUIRE((a.parts == 1 || a.parts == 2) && a.N % a.parts == 0, "linear_fp8: %d rows in %d parts", a.N, a.parts);
-  if (a.M == 0) return ATMA_OK;
+  const atma_fp8_args& f = *args;
+  ATMA_REQUIRE(f.form == 0 || f.form == 1, "linear_fp8: unknown form %d", f.form);
+  ATMA_REQUIRE(f.form == 1 || f.dtype == ATMA_F32 || f.dtype == ATMA_BF16, "linear_fp8: unsupported dtype %d", f.dtype);
+  ATMA_REQUIRE(f.M >= 0 && f.M <= (1 << 28) && f.N > 0 && f.N <= (1 << 24) && f.N % (f.form + 1) == 0 && f.K > 0 && f.K <= (1 << 24),
+               "linear_fp8: bad shape (%d, %d, %d)", f.M, f.N, f.K);
+  ATMA_REQUIRE(f.groups > 0 && f.groups <= kMaxGroups && (f.starts != nullptr || f.groups == 1) && (int64_t)f.groups * f.N <= INT32_MAX - kBM,
+               "linear_fp8: %d groups of %d rows, or without their rows", f.groups, f.N);
+  if (f.M == 0) return ATMA_OK;
   auto al16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
-  ATMA_REQUIRE(a.x != nullptr && a.w != nullptr && a.out != nullptr && a.x_scales != nullptr && a.w_scales != nullptr, "linear_fp8: null tensors");
-  ATMA_REQUIRE(al16(a.x) && al16(a.w) && a.x_rs % 16 == 0 && a.w_rs % 16 == 0 && a.x_rs >= a.K && a.w_rs >= a.K,
+  ATMA_REQUIRE(f.x != nullptr && f.w != nullptr && f.out != nullptr && f.x_scales != nullptr && f.w_scales != nullptr, "linear_fp8: null tensors");
+  ATMA_REQUIRE(al16(f.x) && al16(f.w) && f.x_rs % 16 == 0 && f.w_rs % 16 == 0 && f.x_rs >= f.K && f.w_rs >= f.K,
                "linear_fp8: rows of x and of the weight must start on 16-byte boundaries");
-  ATMA_REQUIRE(a.out_rs >= a.N && a.xs_bs >= a.M, "linear_fp8: overlapping rows");
-  const dim3 grid((unsigned)(a.M / kTile + (a.groups < a.M ? a.groups : a.M)), (unsigned)((a.N + kTile - 1) / kTile));
-  ATMA_REQUIRE(grid.y <= 65535, "linear_fp8: N=%d", a.N);
+  const int width = f.N / (f.form + 1);
+  ATMA_REQUIRE(f.out_rs >= width && f.xs_bs >= f.M, "linear_fp8: overlapping rows");
+  ATMA_REQUIRE(f.form == 0 || (f.out_scales != nullptr && f.os_bs >= f.M && al16(f.out) && f.out_rs % 16 == 0),
+               "linear_fp8: results in 8 bits need scales and rows that start on 16-byte boundaries");
+  const Args a{f.x_scales, f.w_scales, f.out, f.out_scales, f.starts, f.xs_bs, f.out_rs, f.os_bs, f.M, width, f.K, f.groups, (width + 127) / 128,
+               (f.K + 127) / 128, al16(f.out) && f.out_rs * (f.dtype == ATMA_F32 ? 4 : 2) % 16 == 0};
   cudaStream_t st = (cudaStream_t)stream;
-  if (a.dtype == ATMA_F32) linear_fp8_kernel<float><<<grid, 256, 0, st>>>(a);
-  else linear_fp8_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a);
-  return launch_status("linear_fp8");
+  if (f.form == 1) return launch<float, true>(f, a, st);
+  return f.dtype == ATMA_F32 ? launch<float, false>(f, a, st) : launch<__nv_bfloat16, false>(f, a, st);
 }

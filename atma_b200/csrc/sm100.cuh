@@ -250,5 +250,7 @@ PFN_encodeTiled get_encode_tiled();
 // 128-byte swizzle, out-of-bounds elements read as zero.  Returns 0 on success.
 int make_tmap_16bit_4d(CUtensorMap* out, const void* base, int is_bf16, const uint64_t dims[4],
                        const int64_t strides[3], const uint32_t box[4]);
+// The same of bytes: rows of `cols` that are `row_stride` apart, boxes of 128 columns.
+int make_tmap_8bit_rows(CUtensorMap* out, const void* base, uint64_t rows, int64_t row_stride, uint64_t cols, uint32_t box_rows);
 
 }  // namespace atma

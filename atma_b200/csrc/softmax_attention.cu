@@ -6,6 +6,7 @@
 // the scores, and vdim / 32 value channels for the weighted sum, so the softmax statistics of a row are warp reductions.
 #include "linear_act.cuh"
 #include "linear_f32.cuh"
+#include "linear_fp8.cuh"
 #include "softmax_attention.cuh"
 
 namespace atma {
@@ -227,12 +228,13 @@ extern "C" int64_t atma_softmax_decode_scratch_floats(int n_seqs, int H, int map
 
 extern "C" int atma_decoder_device_status(int* status) {
   ATMA_REQUIRE(status != nullptr, "decoder_device_status: null out pointer");
-  int a = 0, b = 0, c = 0, d = 0, e = 0;
+  int a = 0, b = 0, c = 0, d = 0, e = 0, f = 0;
   int rc = softmax_sm100_status_fetch_and_clear(&a);
   if (rc == ATMA_OK) rc = delta_sm100_status_fetch_and_clear(&b);
   if (rc == ATMA_OK) rc = linear_f32_status_fetch_and_clear(&c);
   if (rc == ATMA_OK) rc = softmax_tf32_status_fetch_and_clear(&d);
   if (rc == ATMA_OK) rc = linear_act_status_fetch_and_clear(&e);
-  *status = a | b | c | d | e;
+  if (rc == ATMA_OK) rc = linear_fp8_status_fetch_and_clear(&f);
+  *status = a | b | c | d | e | f;
   return rc;
 }

@@ -83,9 +83,7 @@ def expert_mlp(x, w_gate_up, w_down, routes, add=None, dtype=torch.bfloat16):
     mine = _new_rows(n, width, dev)
     _check(lib.atma_scatter_rows_fp8(x.values.data_ptr(), _row_stride(x.values), x.scales.data_ptr(), _scale_stride(x.scales), routes.place.data_ptr(), top_k,
                                      mine.values.data_ptr(), _row_stride(mine.values), mine.scales.data_ptr(), n, tokens, width, _lib.stream_ptr()))
-    z = _product(mine, w_gate_up, torch.empty((n, 2 * ff), device=dev), routes.starts, experts, 2)
-    act = _new_rows(n, ff, dev)
-    _check(lib.atma_gelu_gate_fp8(z.data_ptr(), z.stride(0), act.values.data_ptr(), _row_stride(act.values), act.scales.data_ptr(), n, n, ff, _lib.stream_ptr()))
+    act = _product(mine, w_gate_up, _new_rows(n, ff, dev), routes.starts, experts)
     y = _product(act, w_down, torch.empty((n, width), device=dev, dtype=dtype), routes.starts, experts)
     _check(lib.atma_combine_experts(y.data_ptr(), routes.place.data_ptr(), routes.weights.data_ptr(), None if add is None else add.data_ptr(), out.data_ptr(),
                                     tokens, top_k, width, _lib.DTYPE_CODE[dtype], _lib.stream_ptr()))

@@ -193,13 +193,17 @@ def residual_norms_fp8(x, y, weights, eps, offset=1.0, out=None, plain=False):
     return [(r, h if i == len(rows) - 1 else None) for i, r in enumerate(rows)]
 
 
-def _product(x, w, out, starts=None, groups=1, parts=1):
-    a = _lib.Fp8Args()
+def _product(x, w, out, starts=None, groups=1):
+    """x w^T into ``out``: a matrix, or Fp8Rows for the gelu-gated form."""
+    a, gated = _lib.Fp8Args(), isinstance(out, Fp8Rows)
     a.x, a.x_rs, a.x_scales, a.xs_bs = x.values.data_ptr(), _row_stride(x.values), x.scales.data_ptr(), _scale_stride(x.scales)
     a.w, a.w_rs, a.w_scales = w.values.data_ptr(), _row_stride(w.values), w.scales.data_ptr()
-    a.out, a.out_rs = out.data_ptr(), out.stride(0) if out.shape[0] > 1 else out.shape[1]
+    (a.M, n), a.K, a.groups, a.form = out.shape, x.shape[1], groups, int(gated)
+    if gated:
+        a.N, a.out, a.out_rs, a.out_scales, a.os_bs = 2 * n, out.values.data_ptr(), _row_stride(out.values), out.scales.data_ptr(), _scale_stride(out.scales)
+    else:
+        a.N, a.out, a.out_rs, a.dtype = n, out.data_ptr(), out.stride(0) if out.shape[0] > 1 else n, _lib.DTYPE_CODE[out.dtype]
     a.starts = None if starts is None else starts.data_ptr()
-    a.M, a.N, a.K, a.groups, a.parts, a.dtype = out.shape[0], out.shape[1], x.shape[1], groups, parts, _lib.DTYPE_CODE[out.dtype]
     _check(_lib.load_decoder().atma_linear_fp8(ctypes.byref(a), _lib.stream_ptr()))
     return out
 
@@ -218,3 +222,13 @@ def linear_fp8(x, weight, out=None, dtype=torch.bfloat16):
     elif out.shape != (n, N) or out.dtype not in _TYPES or out.stride(1) != 1 and N > 1 or out.stride(0) < N and n > 1:
         raise ValueError("out must have the result's shape, contiguous rows and type bfloat16 or float32")
     return _product(x, weight, out)
+
+
+def gelu_gated_linear_fp8(x, weight):
+    """gelu_tanh(x @ weight[0].T) * (x @ weight[1].T) of rows (rows, K) and a weight (2, N, K) in 8 bits, back in 8 bits: Fp8Rows
+    (rows, N).  Everything between is fp32."""
+    if not isinstance(x, Fp8Rows) or not isinstance(weight, Fp8Weight) or weight.values.ndim != 3 or weight.shape[0] != 2 or \
+            weight.shape[2] != x.shape[1] or 0 in weight.shape:
+        raise ValueError("gelu_gated_linear_fp8 takes Fp8Rows (rows, K) and an Fp8Weight (2, N, K)")
+    _here(x.values, weight.values)
+    return _product(x, weight, _new_rows(x.shape[0], weight.shape[1], x.values.device))

@@ -155,25 +155,24 @@ int atma_delta_step(const atma_delta_args* args, const void* norm_w, void* out, 
 int atma_quantize_rows(const void* x, int64_t x_rs, void* q, int64_t q_rs, float* scales, int64_t s_bs, int rows, int width,
                        int dtype, void* stream);
 
-/* gelu_tanh(z[:, :width]) * z[:, width:] of fp32 rows to 8 bits. */
-int atma_gelu_gate_fp8(const float* z, int64_t z_rs, void* q, int64_t q_rs, float* scales, int64_t s_bs, int rows, int width,
-                       void* stream);
-
 /* atma_residual_norms with results in 8 bits: x + y (y NULL = nothing to add) goes to x_out (NULL = not stored, may be
  * x); of every non-NULL w the norm goes to q and s and, where h is not NULL, to h in the activation dtype. */
 int atma_residual_norms_fp8(const float* x, const void* y, float* x_out, const void* w1, void* q1, float* s1, void* h1,
                             const void* w2, void* q2, float* s2, void* h2, int rows, int D, int64_t q_rs, int64_t s_bs,
                             float eps, float offset, int dtype, void* stream);
 
-/* out[m][n] = sum over b of x_scales[b][m] w_scales[n / 128][b] * (x[m], w[n] over block b), summed in fp32.
- * groups > 1: the weight holds `groups` matrices of N rows, and rows starts[g] .. starts[g + 1] - 1 of x take the g-th.
- * parts = 2: a matrix is two of N / 2 rows, each with blocks of its own (scales [groups][parts][..][..]). */
+/* Products of rows and weights in 8 bits, summed in fp32.
+ *   form 0: out[m][n] = sum over b of x_scales[b][m] w_scales[n / 128][b] * (x[m], w[n] over block b), in dtype
+ *   form 1: w is two matrices of N / 2 rows, each with blocks of its own; out (M, N / 2) = gelu_tanh(first) * second in 8 bits,
+ *           out_scales[b * os_bs + m]
+ * starts: the weight holds `groups` (at most 512) such matrices or pairs, and rows starts[g] .. starts[g + 1] - 1 of x
+ * take the g-th; rows of none are left as they were. */
 typedef struct {
   const void* x; int64_t x_rs; const float* x_scales; int64_t xs_bs;
   const void* w; int64_t w_rs; const float* w_scales;
-  void* out; int64_t out_rs;         /* dtype ATMA_F32 or ATMA_BF16 */
+  void* out; int64_t out_rs; float* out_scales; int64_t os_bs;
   const int32_t* starts;             /* [groups + 1]; NULL = one group of M rows */
-  int M, N, K, groups, parts, dtype;
+  int M, N, K, groups, form, dtype;
 } atma_fp8_args;
 int atma_linear_fp8(const atma_fp8_args* args, void* stream);
 

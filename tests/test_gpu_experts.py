@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import fp8 as O
-from tests.test_gpu_fp8 import loud, ops, rand, weight8
+from tests.test_gpu_fp8 import loud, ops, product_error, rand, weight8
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
@@ -134,7 +134,7 @@ def test_expert_mlp(tokens, n, k, width, ff, dtype):
     add = rand((tokens, width), 4, dtype=dtype)
     for plus in (None, add):
         y = e.expert_mlp(x, w_in, w_out, routes, add=None if plus is None else plus.cuda(), dtype=dtype)
-        err = (max(width, ff) + 8) * 2.0 ** -23
+        err = product_error(max(width, ff))
         want, off, most = O.expert_mlp(O.wide_rows(*O.quantize(h.double())), [in_wide[2 * i:2 * i + 2] for i in range(n)], out_wide, routes.ids.tolist(),
                                        routes.weights.double().tolist(), err)
         if plus is not None:
@@ -156,7 +156,7 @@ def test_expert_mlp_where_all_tokens_go_to_one_expert_and_others_have_none():
     assert routes.starts.tolist() == [0] * 5 + [260] * 5
     y = e.expert_mlp(f.quantize_rows(h.cuda()), w_in, w_out, routes, dtype=torch.float32)
     want, off, most = O.expert_mlp(O.wide_rows(*O.quantize(h.double())), [in_wide[2 * i:2 * i + 2] for i in range(9)], out_wide, routes.ids.tolist(),
-                                   routes.weights.double().tolist(), 152 * 2.0 ** -23)
+                                   routes.weights.double().tolist(), product_error(144))
     assert ((y.cpu().double() - want).abs() <= off + 4 * U * (most + off)).all()
 
 

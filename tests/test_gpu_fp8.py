@@ -4,7 +4,8 @@ What may be off, with u = 2^-24 (half a step of fp32):
   quantize_rows   nothing: scale and value are defined by one rounding each
   norms           the sum by u; a norm by 64 u: its sum of squares has at most 32 + 5 + 8 additions one behind another (half of that in the
                   root), six roundings follow.  A value of 8 bits moves over a border only where fp64's quotient is that near to one
-  products        2 u for every addition, of the largest partial sum: (K + 8) 2^-23 |x| |w|^T; 2^-8 more in bfloat16
+  products        2 u for every addition inside of a block of 128 columns, whose partial sums its own |x| |w|^T bounds, then one addition for
+                  every block, and three roundings of its scale: (2 * 128 + blocks + 3) u |x| |w|^T; 2^-8 more in bfloat16
 """
 
 import pytest
@@ -143,9 +144,13 @@ def test_residual_norms_fp8_in_place_without_y_and_skipped():
     assert not torch.equal(c.scales, d.scales)
 
 
+def product_error(K):
+    return (2 * min(K, 128) + -(-K // 128) + 3) * U
+
+
 def product_bound(x, w, dtype):
     want = x @ w.t()
-    off = (x.shape[1] + 8) * 2.0 ** -23 * (x.abs() @ w.abs().t())
+    off = product_error(x.shape[1]) * (x.abs() @ w.abs().t())
     return want, off + (torch.finfo(dtype).eps / 2 * (want.abs() + off) if dtype != torch.float32 else 0)
 
 
@@ -230,3 +235,38 @@ def test_products_in_a_graph_and_on_another_stream(M):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(got, -want)
+
+
+@pytest.mark.parametrize("M, N, K", [(1, 1, 16), (2, 130, 64), (16, 256, 512), (16, 128, 2048), (31, 200, 256), (64, 100, 1024), (100, 136, 300), (128, 384, 128),
+                                     (129, 200, 256), (300, 264, 520), (520, 130, 1000)])
+def test_gelu_gated_linear_fp8(M, N, K):
+    f = ops()
+    x, xw = rows8(rand((M, K), M))
+    w, (gate, up) = weight8((2, N, K), N)
+    r = f.gelu_gated_linear_fp8(x, w)
+    assert r.shape == (M, N)
+    err = product_error(K)
+    g, u = xw @ gate.t(), xw @ up.t()
+    eg, eu = err * (xw.abs() @ gate.abs().t()), err * (xw.abs() @ up.abs().t())
+    a = O.gelu_tanh(g) * u
+    ea = 1.13 * eg * (u.abs() + eu) + O.gelu_tanh(g).abs() * eu + 2e-5 * a.abs()
+    q, s = O.quantize(a)
+    es = torch.stack([ea[:, b * 128:(b + 1) * 128].amax(1) / 448 for b in range(s.shape[1])], 1) + U * s
+    assert ((r.scales.cpu().double() - s).abs() <= es).all()
+    wide = lambda t: t.repeat_interleave(128, 1)[:, :N]
+    ratio = a / wide(s)
+    off = (ea + ratio.abs() * wide(es)) / wide(s)
+    mine = r.values.cpu().double()
+    assert ((mine - ratio).abs() <= O.step_at(mine) / 2 * 1.0001 + off + O.step_at(ratio) * (off > 0) * 0.5).all()
+    near = (O.to_e4m3(ratio - off) != O.to_e4m3(ratio + off))
+    assert (near | (mine == q)).all()
+
+
+def test_products_leave_no_status():
+    """The bounded waits of the tensor-core kernels: none of this file's launches ran one out."""
+    from atma_b200 import decoder_ops
+    f = ops()
+    x, _ = rows8(rand((300, 256), 1))
+    w, _ = weight8((256, 256), 2)
+    f.linear_fp8(x, w), f.linear_fp8(x[:7], w)
+    assert decoder_ops.device_status() == 0
