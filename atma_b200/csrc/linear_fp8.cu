@@ -7,8 +7,14 @@
 // half of TMEM.  Sums are fp32 all along.
 //
 // Many rows (linear_fp8_pair_kernel): two SMs share a tile of 256 rows x 256 columns of results (cta_group::2: each holds its 128 rows of x
-// and half of the weight's rows, so that a block is 32 KB a CTA for 512 clocks of products).  Eight warps a CTA keep 128 sums a thread;
-// a block costs them 256 clocks of reading TMEM and as many of fma at most.
+// and half of the weight's rows, so that a block is 32 KB a CTA for 512 clocks of products).  Eight warps a CTA keep 128 sums a thread.
+//   warp 0 TMA, warps 1 and 3 products (of the first CTA, for both; 128 columns each), warp 2 scales, warps 4-11 sums and results.
+// Bound by the way from a product to the next one in its place: they are half a block's (128 columns, two places each), so that its 256
+// clocks and what four warps take to read them (300), plus 570 for the barriers between them, share two blocks' 1024.  8192 x 8192 x 4096
+// (1.25 GHz, the clock that the power leaves): 242 us, 2270 TFLOP/s; the same with whole blocks in two places 250; with a release at cluster
+// scope at every block 605; with scales loaded one block ahead by the warps themselves 13 more; products alone 190, 2880 TFLOP/s.  Tried
+// and slower: 16 warps of 64 sums (276 to 340: more waits than sums), 16 columns of TMEM at a time (248), every warp on both halves
+// (266), the next block's wait and first load in front of the last sums (254).
 //
 // Few rows (linear_fp8_rows_kernel): the weight's rows are the tensor core's rows, 128 a tile, and the tokens its columns, 16 to 64, so
 // that a stage is all weight.  Bound by reading that: two CTAs an SM with 100 KB of copies in flight each.  Where a dense product has too few
@@ -101,20 +107,38 @@ __device__ __forceinline__ bool any_gave_up(bool mine) {
   return any != 0;
 }
 
+// Scales come by a warp of their own, eight blocks ahead over all tiles: a load that the sums' warps ask for one block ahead is not there
+// in time (a block of many rows takes 500 clocks, a load twice that).
+constexpr int kAhead = 3, kTogether = 4;                   // groups of blocks, blocks of a group
+
+__device__ __forceinline__ void copy_word(float* to, const float* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void arrive_behind_copies(uint64_t* bar) {              // of this thread
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
 // ---- many rows -------------------------------------------------------------------------------------------
 constexpr int kStages = 5, kStageBytes = 2 * kPlane;
 constexpr int kSumWarps = 8, kPairThreads = 128 + 32 * kSumWarps;
-constexpr int kStaging = 32 * 128;                          // bytes of a warp's 32 rows x 128 bytes of results
+constexpr int kChunk = 32;                                  // columns of TMEM that a thread loads at a time
+constexpr int kStaging = 32 * 64;                           // bytes of a warp's 32 rows x 64 bytes of results
 constexpr int kPairSmem = kStages * kStageBytes + kSumWarps * kStaging + 1024;
 constexpr int kBeside = 8;
 
-// 32 sums of a thread's row += scale * the products in r.
-__device__ __forceinline__ void add_scaled(uint64_t* sum, uint32_t* r, float scale) {
+__device__ __forceinline__ void fma_chunk(uint64_t* sum, uint32_t (&r)[kChunk], float scale) {
   const uint64_t s2 = pack2(scale, scale);
 #pragma unroll
-  for (int i = 0; i < 32; ++i) reg_fence(r[i]);
-#pragma unroll
-  for (int i = 0; i < 16; ++i) sum[i] = fma2(pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), s2, sum[i]);
+  for (int i = 0; i < kChunk / 2; ++i) sum[i] = fma2(pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), s2, sum[i]);
+}
+// One lane's arrival without a branch: the loads in front of it were the whole warp's.
+__device__ __forceinline__ void arrive_cluster_if(bool mine, uint32_t bar) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %1, 0;\n\t@p mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n\t}"
+               ::"r"(bar), "r"((int)mine) : "memory");
+}
+__device__ __forceinline__ bool mbar_wait_lean(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  if (__builtin_expect(__all_sync(0xffffffffu, mbar_try_wait(bar, parity)), 1)) return true;
+  return mbar_wait_warp(bar, parity, abort);
 }
 
 template <typename T, bool kGated>
@@ -122,11 +146,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ Args a) {
   constexpr int kTileN = kGated ? 128 : 256;                // columns of results of a tile
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];      // full and acc_empty: the first CTA's are used
+  __shared__ uint64_t full[kStages], empty[kStages], acc_full[4], acc_empty[4];      // full and acc_empty: the first CTA's are used
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort_v;
   __shared__ int s_first[kMaxGroups + 1];
   __shared__ float s_most[kGated ? 2 : 1][2][kGated ? 128 : 1];
+  __shared__ uint64_t sc_full[kAhead], sc_empty[kAhead];
+  __shared__ float s_scale[kAhead][kTogether][kBM + 2];     // of the rows, then of the weight's two blocks
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t rank;
@@ -139,8 +165,9 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
   }
   if (warp == 2) count_tiles(s_first, a, 2 * kBM);
   if (tid == 32) {
-    for (int i = 0; i < kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 2 * kSumWarps); }
+    for (int i = 0; i < kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 2); }
+    for (int i = 0; i < 4; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], kSumWarps); }
+    for (int i = 0; i < kAhead; ++i) { mbar_init(&sc_full[i], 32); mbar_init(&sc_empty[i], kSumWarps); }
     s_abort_v = 0;
     fence_barrier_init();
   }
@@ -161,7 +188,8 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
         for (int tile = pair; tile < tiles && ok; tile += pairs) {
           const Place p = place_of(tile, s_first, a, 2 * kBM, kTileN, n_tiles, kBeside);
           const int xr = p.m0 + (int)rank * kBM;
-          const int wr = kGated ? (2 * p.group + (int)rank) * a.width + p.n0 : p.group * a.width + p.n0 + (int)rank * kBM;
+          // 64 rows of the weight for either half of the tile's columns
+          const int wr = kGated ? (2 * p.group + (int)rank) * a.width + p.n0 : p.group * a.width + p.n0 + (int)rank * 64, next = kGated ? 64 : 128;
           for (int it = 0; it < a.kb; ++it, ++n) {
             const uint32_t st = n % kStages;
             if (n >= kStages && !(ok = mbar_wait(&empty[st], (n / kStages - 1) & 1, abort))) break;
@@ -170,6 +198,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
             const uint32_t bar = in_first(smem_u32(&full[st]));
             tma_load_pair(to, &tm_x, bar, it * kBK, xr);
             tma_load_pair(to + kPlane, &tm_w, bar, it * kBK, wr);
+            tma_load_pair(to + kPlane + kPlane / 2, &tm_w, bar, it * kBK, wr + next);
           }
         }
         // whatever the others do, the CTA does not end before its copies have landed and the products that read them are done
@@ -177,85 +206,106 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
         for (uint32_t i = n > kStages ? n - kStages : 0; i < n; ++i)
           if (!mbar_wait(&empty[i % kStages], (i / kStages) & 1, &alone)) { *abort = 1; break; }
       }
-    } else if (warp == 1) {
+    } else if (warp == 1 || warp == 3) {    // a half of the results each
       if (rank == 0 && elect_one()) {
-        constexpr uint32_t idesc = make_idesc(2 * kBM, 2 * kBM, 0, 0, 0);
+        constexpr uint32_t idesc = make_idesc(2 * kBM, kBM, 0, 0, 0);
+        const int h = warp >> 1;
+        const uint64_t first = make_sdesc_sw128(smem_u32(smem), 16, 1024);
         uint32_t n = 0;
         bool ok = true;
         for (int tile = pair; tile < tiles && ok; tile += pairs) {
           for (int it = 0; it < a.kb; ++it, ++n) {
-            const uint32_t st = n % kStages, buf = n & 1;
-            if (n >= 2 && !(ok = mbar_wait(&acc_empty[buf], (n / 2 - 1) & 1, abort))) break;
+            const uint32_t st = n % kStages, slot = 2 * (n & 1) + h;
             if (!(ok = mbar_wait(&full[st], (n / kStages) & 1, abort))) break;
+            if (n >= 2 && !(ok = mbar_wait(&acc_empty[slot], (n / 2 - 1) & 1, abort))) break;
             tc_fence_after();
-            const uint32_t at = smem_u32(smem + st * kStageBytes), d = tmem + buf * 2 * kBM;
+            const uint64_t x = first + st * (kStageBytes >> 4), w = x + ((kPlane + h * kPlane / 2) >> 4);      // descriptors count in 16 bytes
 #pragma unroll
-            for (int k = 0; k < kBK / 32; ++k)
-              mma_pair_8bit(d, make_sdesc_sw128(at + 32 * k, 16, 1024), make_sdesc_sw128(at + kPlane + 32 * k, 16, 1024), idesc, k > 0);
+            for (int k = 0; k < kBK / 32; ++k) mma_pair_8bit(tmem + slot * kBM, x + 2 * k, w + 2 * k, idesc, k > 0);
+            commit_pair(&acc_full[slot]);
             commit_pair(&empty[st]);
-            commit_pair(&acc_full[buf]);
           }
         }
       }
+    } else if (warp == 2) {
+      uint32_t n = 0;
+      bool ok = true;
+      for (int tile = pair; tile < tiles && ok; tile += pairs) {
+        const Place p = place_of(tile, s_first, a, 2 * kBM, kTileN, n_tiles, kBeside);
+        const int row0 = p.m0 + (int)rank * kBM + lane, block = p.n0 / 128;
+        // the blocks of the weight's rows that meet in the tile: two neighbours, or one of either half
+        const float* ws = a.w_scales + (kGated ? (int64_t)(2 * p.group + (lane & 1)) * a.nb + block
+                                               : (int64_t)p.group * a.nb + min(block + (lane & 1), a.nb - 1)) * a.kb;
+        for (int i0 = 0; i0 < a.kb; i0 += kTogether, ++n) {
+          const uint32_t at = n % kAhead;
+          if (n >= kAhead && !(ok = mbar_wait_warp(&sc_empty[at], (n / kAhead - 1) & 1, abort))) break;
+          for (int it = i0; it < min(i0 + kTogether, a.kb); ++it) {
+#pragma unroll
+            for (int i = 0; i < kBM; i += 32) copy_word(&s_scale[at][it - i0][i + lane], a.x_scales + it * a.xs_bs + min(row0 + i, a.M - 1));
+            if (lane < 2) copy_word(&s_scale[at][it - i0][kBM + lane], ws + it);
+          }
+          arrive_behind_copies(&sc_full[at]);
+        }
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");      // nothing lands in a CTA that is gone
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int w = warp - 4, quarter = warp & 3, side = w >> 2;
     uint8_t* s = smem + kStages * kStageBytes + w * kStaging;
-    uint32_t n = 0, turn = 0;
+    const uint32_t acc_empty_there = in_first(smem_u32(&acc_empty[0]));
+    uint32_t n = 0, g = 0, turn = 0;        // blocks and groups of scales so far
     bool ok = true;
     for (int tile = pair; tile < tiles && ok; tile += pairs, turn ^= 1) {
       const Place p = place_of(tile, s_first, a, 2 * kBM, kTileN, n_tiles, kBeside);
       const int row0 = p.m0 + (int)rank * kBM + 32 * quarter, row = row0 + lane;
-      // gated: 64 columns of either half a thread, the halves 128 columns of TMEM apart; else 128 columns of results
-      const int c0 = kGated ? 64 * side : 128 * side, behind = kGated ? 128 : 64;
-      const float* xs = a.x_scales + min(row, a.M - 1);
-      const float* ws = a.w_scales + (kGated ? ((int64_t)(2 * p.group) * a.nb + p.n0 / 128) : ((int64_t)p.group * a.nb + min(p.n0 / 128 + side, a.nb - 1))) * a.kb;
-      const float* us = ws + (kGated ? (int64_t)a.nb * a.kb : 0);
+      const int c0 = 128 * side;              // gated: 64 of either half of the weight; else a block's
       uint64_t sum[64];
 #pragma unroll
       for (int i = 0; i < 64; ++i) sum[i] = 0;
-      float fx = xs[0], fw = ws[0], fu = us[0];
-      for (int it = 0; it < a.kb; ++it, ++n) {
-        const uint32_t buf = n & 1, at = tmem + (uint32_t(32 * quarter) << 16) + buf * 2 * kBM + c0;
-        const float sw = fx * fw, su = fx * fu;
-        if (it + 1 < a.kb) { fx = xs[(int64_t)(it + 1) * a.xs_bs]; fw = ws[it + 1]; fu = us[it + 1]; }
-        if (!(ok = mbar_wait_warp(&acc_full[buf], (n / 2) & 1, abort))) break;
-        tc_fence_after();
-        uint32_t r0[32], r1[32];
-        tmem_ld32_nowait(at, r0);
-        tmem_ld_wait();
-        tmem_ld32_nowait(at + 32, r1);
-        add_scaled(sum, r0, sw);
-        tmem_ld_wait();
-        tmem_ld32_nowait(at + behind, r0);
-        add_scaled(sum + 16, r1, sw);
-        tmem_ld_wait();
-        tmem_ld32_nowait(at + behind + 32, r1);
-        add_scaled(sum + 32, r0, su);
-        tmem_ld_wait();
+      for (int i0 = 0; i0 < a.kb && ok; i0 += kTogether, ++g) {
+        const uint32_t sc = g % kAhead;
+        if (!(ok = mbar_wait_lean(&sc_full[sc], (g / kAhead) & 1, abort))) break;
+        const int blocks = min(kTogether, a.kb - i0);
+        for (int it = 0; it < blocks; ++it, ++n) {
+          const uint32_t buf = n & 1, slot = 2 * buf + side, at = tmem + (uint32_t(32 * quarter) << 16) + slot * kBM;
+          const float fx = s_scale[sc][it][32 * quarter + lane], fw = s_scale[sc][it][kBM + (kGated ? 0 : side)], fu = s_scale[sc][it][kBM + 1];
+          if (!(ok = mbar_wait_lean(&acc_full[slot], (n / 2) & 1, abort))) break;
+          tc_fence_after();
+          uint32_t r[2][kChunk];
+          tmem_ld32_nowait(at, r[0]);
+          const float sw = fx * fw, su = kGated ? fx * fu : sw;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) reg_fence(r1[i]);
-        tc_fence_before();
+          for (int c = 0; c < 128; c += kChunk) {
+            uint32_t(&now)[kChunk] = r[c / kChunk & 1];
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) reg_fence(now[i]);
+            const int next = c + kChunk;
+            if (next < 128) tmem_ld32_nowait(at + next, r[next / kChunk & 1]);
+            else {
+              tc_fence_before();
+              arrive_cluster_if(lane == 0, acc_empty_there + slot * 8);
+            }
+            fma_chunk(sum + c / 2, now, c >= 64 ? su : sw);
+          }
+        }
         __syncwarp();
-        if (lane == 0) arrive_cluster(in_first(smem_u32(&acc_empty[buf])));
-        add_scaled(sum + 48, r1, su);
+        if (lane == 0) mbar_arrive(&sc_empty[sc]);
       }
-      if constexpr (!kGated)
-        if (!ok) break;
-      if constexpr (kGated) {
+      if constexpr (kGated) {               // whether it goes on is decided by all warps together, below
         const int f0 = p.n0 + 64 * side;
         float v[64], most = 0.f;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float2 g = unpack2(sum[i]), u = unpack2(sum[32 + i]);
-          v[2 * i] = f0 + 2 * i < a.width ? gelu_tanh_16(g.x) * u.x : 0.f;
-          v[2 * i + 1] = f0 + 2 * i + 1 < a.width ? gelu_tanh_16(g.y) * u.y : 0.f;
-          most = max_nan(most, max_nan(fabsf(v[2 * i]), fabsf(v[2 * i + 1])));
+        for (int i = 0; i < 64; i += 2) {
+          const float2 g = unpack2(sum[i / 2]), u = unpack2(sum[32 + i / 2]);
+          v[i] = f0 + i < a.width ? gelu_tanh_16(g.x) * u.x : 0.f;
+          v[i + 1] = f0 + i + 1 < a.width ? gelu_tanh_16(g.y) * u.y : 0.f;
+          most = max_nan(most, max_nan(fabsf(v[i]), fabsf(v[i + 1])));
         }
         // a block's 128 columns are two warps': its largest value through shared memory, in turns of two
         s_most[turn][side][32 * quarter + lane] = most;
-        if (any_gave_up<256>(!ok || *abort)) break;
+        if (any_gave_up<32 * kSumWarps>(!ok || *abort)) break;
         const float scale = fp8_scale(max_nan(s_most[turn][0][32 * quarter + lane], s_most[turn][1][32 * quarter + lane]));
         if (row < p.m1) {
           if (side == 0) a.out_scales[(int64_t)(p.n0 / 128) * a.os_bs + row] = scale;
@@ -276,12 +326,13 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
           }
         }
       } else {
-        constexpr int kCols = 128 / sizeof(T), kPer = 16 / sizeof(T);              // columns of a chunk of 128 bytes, of a piece of 16
+        if (!ok) break;
+        constexpr int kCols = 64 / sizeof(T), kPer = 16 / sizeof(T);               // columns of a chunk of 64 bytes, of a piece of 16
         T* out = static_cast<T*>(a.out);
 #pragma unroll
         for (int chunk = 0; chunk < 128 / kCols; ++chunk) {
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
+          for (int q = 0; q < 4; ++q) {
             alignas(16) T o[kPer];
 #pragma unroll
             for (int j = 0; j < kPer; j += 2) {
@@ -289,13 +340,13 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
               o[j] = from_f32<T>(f.x);
               o[j + 1] = from_f32<T>(f.y);
             }
-            *reinterpret_cast<uint4*>(s + lane * 128 + ((q ^ (lane & 7)) << 4)) = *reinterpret_cast<const uint4*>(o);
+            *reinterpret_cast<uint4*>(s + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)) = *reinterpret_cast<const uint4*>(o);
           }
           __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {     // four rows at a time, 128 bytes each
-            const int r = 4 * i + (lane >> 3), q = lane & 7, col = p.n0 + c0 + chunk * kCols + q * kPer;
-            const uint4 v = *reinterpret_cast<const uint4*>(s + r * 128 + ((q ^ (r & 7)) << 4));
+          for (int i = 0; i < 4; ++i) {     // eight rows at a time, 64 bytes each
+            const int r = 8 * i + (lane >> 2), q = lane & 3, col = p.n0 + c0 + chunk * kCols + q * kPer;
+            const uint4 v = *reinterpret_cast<const uint4*>(s + r * 64 + ((q ^ (r >> 1 & 3)) << 4));
             if (row0 + r >= p.m1) continue;
             T* to = out + (int64_t)(row0 + r) * a.out_rs + col;
             if (a.vec && col + kPer <= a.width) *reinterpret_cast<uint4*>(to) = v;
@@ -600,7 +651,7 @@ int launch(const atma_fp8_args& f, const Args& a, cudaStream_t st) {
   const int each = (a.M + a.groups - 1) / a.groups, nt = each <= 16 ? 16 : each <= 32 ? 32 : each <= 128 ? 64 : 0;
   CUtensorMap x, w;
   int rc = make_tmap_8bit_rows(&x, f.x, a.M, f.x_rs, a.K, nt > 0 ? nt : kBM);
-  if (rc == ATMA_OK) rc = make_tmap_8bit_rows(&w, f.w, (uint64_t)a.groups * f.N, f.w_rs, a.K, kBM);
+  if (rc == ATMA_OK) rc = make_tmap_8bit_rows(&w, f.w, (uint64_t)a.groups * f.N, f.w_rs, a.K, nt > 0 ? kBM : kBM / 2);
   if (rc != ATMA_OK) return rc;
   if (nt == 16) return launch_rows<T, 16, kGated>(x, w, a, st);
   if (nt == 32) return launch_rows<T, 32, kGated>(x, w, a, st);
