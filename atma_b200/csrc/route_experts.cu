@@ -39,6 +39,8 @@ struct RouteArgs {
   int tokens, experts, k, groups, top_groups, chunk, chunks;
   float scale;
   bool sigmoid, renormalize;
+  bool vec;                                 // rows start on 16-byte boundaries
+  bool lanes;                               // choose_fast: groups are 1, 2, 4, .. whole lanes, k is below 32
 };
 
 // floats and doubles as integers in the same order; 0 is below all of them
@@ -179,7 +181,9 @@ __device__ __forceinline__ bool choose(const float (&z)[V], int e0, const RouteA
     const int holder = __ffs(__ballot_sync(0xffffffffu, best == most)) - 1;
     const int e = __shfl_sync(0xffffffffu, e0 + where, holder);
     const float got = (float)__shfl_sync(0xffffffffu, at, holder);
-    if (lane == (n & 31)) { id[n >> 5] = e; score[n >> 5] = got; }
+    if (lane == (n & 31)) {
+      if (n < 32) { id[0] = e; score[0] = got; } else { id[1] = e; score[1] = got; }
+    }
     if (lane == holder) {
 #pragma unroll
       for (int v = 0; v < V; ++v)
@@ -191,7 +195,156 @@ __device__ __forceinline__ bool choose(const float (&z)[V], int e0, const RouteA
 
 template <int V>
 __device__ __noinline__ void choose_in_64(const float (&z)[V], int e0, const RouteArgs& a, int (&id)[2], float (&score)[2]) {
-  choose<double, V, false>(z, e0, a, id, score);
+  if (a.bias == nullptr && a.groups == 1) choose<double, V, true>(z, e0, a, id, score);
+  else choose<double, V, false>(z, e0, a, id, score);
+}
+
+// A lane's words in falling order: odd-even merge sort.
+template <int V>
+__device__ __forceinline__ void sort_words(uint32_t (&w)[V]) {
+#pragma unroll
+  for (int p = 1; p < V; p *= 2)
+#pragma unroll
+    for (int d = p; d > 0; d /= 2)
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i >= d % p && (i - d % p) % (2 * d) < d && i + d < V && i / (2 * p) == (i + d) / (2 * p)) {
+          const uint32_t hi = max(w[i], w[i + d]), lo = min(w[i], w[i + d]);
+          w[i] = hi; w[i + d] = lo;
+        }
+}
+
+// The same in fp32 where every lane's experts are of one group (or there are none), a group is 1, 2, 4, .. lanes and k is small.
+//
+// Keys come from instructions that round more; what they are off by stays below kKeyError, since s (1 - s) |z| and |d| exp(-|d|),
+// d = z - max, are below 0.4.  A key and its expert are one word: the key as an ordered integer without its last bits, the expert there,
+// lower ones larger.  A lane sorts its words once, and a round is one redux over the lanes' first ones.  Rounds go on until k words are
+// taken and the next key is surely below the last; if some of the taken are nearer to one another than that, each lane computes one
+// taken expert's key in fp64 and counts those above it.  Lane `rank` of the result: choice `rank`.  kFull: no lane has places without an expert.
+template <int V, bool kFull>
+__device__ __forceinline__ bool choose_fast(const float (&z)[V], const float (&bias)[V], int e0, const RouteArgs& a, const float* row, int* rank, int* id, float* score) {
+  constexpr uint32_t kPlace = V <= 8 ? 255 : 511;
+  const int lane = threadIdx.x & 31, own = kFull ? V : a.experts - e0;             // the lane's experts, if they are fewer than V
+  const bool exact = a.bias == nullptr && a.groups == 1;     // keys are the logits
+  const float width = exact ? 0.f : kKeyError;
+  float key[V], m = 0.f, sum = 1.f;
+  if (!a.sigmoid) {
+    m = z[0];
+#pragma unroll
+    for (int v = 1; v < V; ++v) m = fmaxf(m, z[v]);          // behind the last expert z is -FLT_MAX
+    m = value_of(warp_most(ordered(m)));
+    sum = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      key[v] = v < own ? expf(z[v] - m) : 0.f;
+      sum += key[v];
+    }
+    sum = warp_add(sum);
+    const float r = 1.f / sum;
+#pragma unroll
+    for (int v = 0; v < V; ++v) key[v] *= r;
+  } else if (!exact) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) key[v] = __fdividef(1.f, 1.f + __expf(-z[v]));
+  }
+  if (exact) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) key[v] = z[v];
+  } else if (a.bias != nullptr) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) key[v] = fmaxf(key[v] + bias[v], -FLT_MAX);         // a NaN becomes -FLT_MAX here
+  }
+  bool out = false;                         // this lane's group goes
+  if (a.groups > 1) {                       // V divides a group here: own is V or less than 1
+    const int lanes = a.experts / a.groups / V, mine = lane & -lanes;
+    float best = key[0], second = -INFINITY;
+#pragma unroll
+    for (int v = 1; v < V; ++v) {
+      second = fmaxf(second, fminf(best, key[v]));
+      best = fmaxf(best, key[v]);
+    }
+    for (int o = 1; o < lanes; o <<= 1) {
+      const float b = __shfl_xor_sync(0xffffffffu, best, o), c = __shfl_xor_sync(0xffffffffu, second, o);
+      second = fmaxf(fmaxf(second, c), fminf(best, b));
+      best = fmaxf(best, b);
+    }
+    const float both = second == -INFINITY ? best : best + second;
+    int above = 0;                          // groups that are better than this lane's
+    float nearest = INFINITY;
+    for (int from = 0; from < a.groups * lanes; from += lanes) {
+      const float other = __shfl_sync(0xffffffffu, both, from);
+      above += other > both;
+      nearest = fminf(nearest, from == mine ? INFINITY : fabsf(other - both));
+    }
+    const bool settled = (nearest > 2.f * width * (fabsf(both) + 1.f) && both > -FLT_MAX) || lane >= a.groups * lanes;
+    if (!__all_sync(0xffffffffu, settled)) return false;
+    out = above >= a.top_groups;
+  }
+  uint32_t word[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    word[v] = (ordered(out ? -FLT_MAX : key[v]) & ~kPlace) | (kPlace - (uint32_t)(e0 + v));
+    if (!kFull && v >= own) word[v] = 0;    // nobody's: below all others
+  }
+  sort_words<V>(word);
+  auto take = [&]() {                       // the largest word that is left
+    const uint32_t most = warp_most(word[0]);
+    if (word[0] == most) {
+#pragma unroll
+      for (int v = 0; v + 1 < V; ++v) word[v] = word[v + 1];
+      word[V - 1] = 0;
+    }
+    return most;
+  };
+  auto apart = [&](uint32_t above, uint32_t below) {         // what the key above is at least, and the one below at most
+    const float p = value_of(above & ~kPlace), q = value_of(below | kPlace);
+    return below == 0 || (exact ? (above & ~kPlace) > (below | kPlace) : p - q > width * (fabsf(p) + 1.f));
+  };
+  uint32_t taken = 0;                       // lane n: word n
+  for (int n = 0; n <= a.k; ++n) {
+    const uint32_t most = take();
+    if (lane == n) taken = most;
+  }
+  int n = a.k;                              // words that are surely above the next one
+  const uint32_t next = __shfl_down_sync(0xffffffffu, taken, 1);
+  const uint32_t near = __ballot_sync(0xffffffffu, lane < a.k && !apart(taken, next));
+  if (near >> (a.k - 1)) {
+    uint32_t last = __shfl_sync(0xffffffffu, taken, n);
+    do {
+      if (++n == 32) return false;
+      const uint32_t most = take();
+      if (lane == n) taken = most;
+      if (apart(last, most)) break;
+      last = most;
+    } while (true);
+  }
+  const int e = lane < n ? (int)(kPlace - (taken & kPlace)) : 0;
+  const float x = fminf(fmaxf(row[e], -FLT_MAX), FLT_MAX);
+  *id = e;
+  *rank = lane < n ? lane : 32;
+  *score = a.sigmoid ? 1.f / (1.f + expf(-x)) : expf(x - m) / sum;
+  if (near) {                               // the same for all lanes
+    double total = 1., f = x;
+    if (!exact) {
+      if (a.sigmoid) {
+        f = 1. / (1. + exp(-(double)x));
+      } else {
+        total = 0.;
+#pragma unroll 1
+        for (int i = lane; i < a.experts; i += 32) total += exp((double)fminf(fmaxf(row[i], -FLT_MAX), FLT_MAX) - (double)m);
+        f = exp((double)x - (double)m) / warp_add(total);
+      }
+      if (a.bias != nullptr) f += isnan(a.bias[e]) ? -INFINITY : a.bias[e];
+    }
+    int above = 0;
+    for (int i = 0; i < n; ++i) {
+      const double g = __shfl_sync(0xffffffffu, f, i);
+      const int h = __shfl_sync(0xffffffffu, e, i);
+      above += g > f || (g == f && h < e);
+    }
+    if (lane < n) *rank = above;
+  }
+  return true;
 }
 
 // ---- places ----------------------------------------------------------------------------------------------
@@ -260,7 +413,7 @@ __device__ void place_entries(OrderShared& s, const RouteArgs& a, int t0, int t1
   }
 }
 
-template <int V>
+template <int V, bool kFull>
 __global__ void __launch_bounds__(kRouteThreads)
 route_experts_kernel(const RouteArgs a) {
   early_start();
@@ -270,28 +423,48 @@ route_experts_kernel(const RouteArgs a) {
   for (int e = tid; e < a.experts; e += kRouteThreads) s_counts[e] = 0;
   __syncthreads();
   const int t0 = blockIdx.x * a.chunk, t1 = min(a.tokens, t0 + a.chunk);
+  float bias[V], next[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) bias[v] = a.bias != nullptr && (kFull || e0 + v < a.experts) ? a.bias[e0 + v] : 0.f;
+  auto bring = [&](int t) {                 // a token's logits, one token ahead
+    const float* row = a.logits + (int64_t)t * a.l_rs;
+    if (V % 4 == 0 && a.vec && (kFull || e0 + V <= a.experts)) {
+#pragma unroll
+      for (int v = 0; v < V; v += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(row + e0 + v);
+        next[v] = f.x; next[(v + 1) % V] = f.y; next[(v + 2) % V] = f.z; next[(v + 3) % V] = f.w;
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) next[v] = kFull || e0 + v < a.experts ? row[e0 + v] : -FLT_MAX;
+    }
+  };
+  if (t0 + warp < t1) bring(t0 + warp);
   for (int t = t0 + warp; t < t1; t += kRouteWarps) {
     const float* row = a.logits + (int64_t)t * a.l_rs;
     float z[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float f = e0 + v < a.experts ? row[e0 + v] : -FLT_MAX;
-      z[v] = fminf(fmaxf(f, -FLT_MAX), FLT_MAX);             // a NaN becomes -FLT_MAX here
-    }
-    int id[2] = {0, 0};
+    for (int v = 0; v < V; ++v) z[v] = fminf(fmaxf(next[v], -FLT_MAX), FLT_MAX);   // a NaN becomes -FLT_MAX here
+    if (t + kRouteWarps < t1) bring(t + kRouteWarps);
+    // choices of this lane and the places they go to; places behind k are not taken
+    int id[2] = {0, 0}, rank[2] = {lane, lane + 32};
     float score[2] = {0.f, 0.f};
-    if (a.bias == nullptr && a.groups == 1) choose<float, V, true>(z, e0, a, id, score);
-    else if (!choose<float, V, false>(z, e0, a, id, score)) choose_in_64<V>(z, e0, a, id, score);
+    if (!a.lanes || !choose_fast<V, kFull>(z, bias, e0, a, row, rank, id, score)) {
+      rank[0] = lane;
+      if (a.lanes || !choose<float, V, false>(z, e0, a, id, score)) choose_in_64<V>(z, e0, a, id, score);
+    } else {
+      rank[1] = a.k;
+    }
     if (a.renormalize) {
-      const float sum = warp_sum(score[0] + score[1]);
+      const float sum = warp_sum((rank[0] < a.k ? score[0] : 0.f) + (rank[1] < a.k ? score[1] : 0.f));
 #pragma unroll
       for (int i = 0; i < 2; ++i) score[i] = sum > 0.f ? score[i] / sum : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      if (lane + 32 * i < a.k) {
-        a.ids[(int64_t)t * a.k + lane + 32 * i] = id[i];
-        a.weights[(int64_t)t * a.k + lane + 32 * i] = score[i] * a.scale;
+      if (rank[i] < a.k) {
+        a.ids[(int64_t)t * a.k + rank[i]] = id[i];
+        a.weights[(int64_t)t * a.k + rank[i]] = score[i] * a.scale;
         atomicAdd(&s_counts[id[i]], 1);                      // whole numbers: any order gives the same
       }
   }
@@ -307,16 +480,26 @@ route_experts_kernel(const RouteArgs a) {
 __global__ void __launch_bounds__(kRouteThreads)
 order_experts_kernel(const RouteArgs a) {
   extern __shared__ uint8_t s_more[];
-  const int tid = threadIdx.x;
+  // the chunks' counts, by as many threads an expert as there are, 16 loads of each under way
+  const int tid = threadIdx.x, each = kRouteThreads / a.experts, e = tid % a.experts, part = tid / a.experts;
+  int32_t* s_sum = reinterpret_cast<int32_t*>(s_more);       // [2][kMaxExperts]
+  for (int i = tid; i < 2 * kMaxExperts; i += kRouteThreads) s_sum[i] = 0;
+  __syncthreads();
   int before = 0, total = 0;
-  if (tid < a.experts) {
-#pragma unroll 8
-    for (int c = 0; c < a.chunks; ++c) {
-      const int n = a.counts[(int64_t)c * a.experts + tid];
+  if (part < each) {
+#pragma unroll 16
+    for (int c = part; c < a.chunks; c += each) {
+      const int n = a.counts[(int64_t)c * a.experts + e];
       if (c < (int)blockIdx.x) before += n;
       total += n;
     }
+    atomicAdd(&s_sum[e], before);
+    atomicAdd(&s_sum[kMaxExperts + e], total);
   }
+  __syncthreads();
+  before = tid < a.experts ? s_sum[tid] : 0;
+  total = tid < a.experts ? s_sum[kMaxExperts + tid] : 0;
+  __syncthreads();                                           // the memory is place_entries' next
   const int t0 = blockIdx.x * a.chunk;
   place_entries(*reinterpret_cast<OrderShared*>(s_more), a, t0, min(a.tokens, t0 + a.chunk), before, total, blockIdx.x == 0);
 }
@@ -324,12 +507,15 @@ order_experts_kernel(const RouteArgs a) {
 // Tokens of a chunk: as few as give every SM one, 32 at least.
 int route_chunk(int tokens) {
   const int sms = sm_count_of_current_device(), n = (tokens + sms - 1) / sms;
+  if (tokens <= 128) return 128;                             // one launch takes less than two
   return n <= 32 ? 32 : (n + 31) / 32 * 32;
 }
 
 template <int V>
-int launch_route(const RouteArgs& a, cudaStream_t st) {
-  auto kernel = route_experts_kernel<V>;
+int launch_route(RouteArgs a, cudaStream_t st) {
+  const int size = a.experts / a.groups;
+  a.lanes = a.k < 32 && (a.groups == 1 || (size % V == 0 && (size / V & (size / V - 1)) == 0));
+  auto kernel = a.experts == 32 * V ? route_experts_kernel<V, true> : route_experts_kernel<V, false>;
   const size_t more = a.chunks == 1 ? sizeof(OrderShared) : 0;
   launch_early(a.tokens, kernel, a.chunks, kRouteThreads, more, st, a);
   return launch_status("route_experts");
@@ -365,7 +551,7 @@ extern "C" int atma_route_experts(const float* logits, int64_t l_rs, const float
   const int chunk = route_chunk(tokens), chunks = (tokens + chunk - 1) / chunk;
   ATMA_REQUIRE(chunks == 1 || scratch != nullptr, "route_experts: no scratch memory");
   const RouteArgs a{logits, l_rs, bias, ids, weights, scratch, order, place, starts, tokens, experts, k, groups, top_groups, chunk, chunks, scale,
-                    sigmoid != 0, renormalize != 0};
+                    sigmoid != 0, renormalize != 0, (reinterpret_cast<uintptr_t>(logits) & 15) == 0 && l_rs % 4 == 0, false};
   int rc;
   if (experts <= 32) rc = launch_route<1>(a, st);
   else if (experts <= 64) rc = launch_route<2>(a, st);

@@ -10,7 +10,7 @@ import torch
 
 from . import _lib
 from .decoder_ops import _check
-from .fp8_ops import Fp8Rows, Fp8Weight, _here, _new_rows, _product, _row_stride, _scale_stride, _TYPES
+from .fp8_ops import Fp8Rows, Fp8Weight, _here, _new_rows, _product, _TYPES
 
 MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 512, 64, 64
 
@@ -43,16 +43,17 @@ def route_experts(logits, top_k, *, score="softmax", bias=None, groups=1, top_gr
         raise ValueError(f"{top_groups} of {groups} groups of {experts} experts (at most {MAX_EXPERTS} in {MAX_GROUPS} groups)")
     if not 0 < top_k <= min(MAX_TOP_K, experts // groups * top_groups):
         raise ValueError(f"{top_k} of {experts // groups * top_groups} experts (at most {MAX_TOP_K})")
-    if logits.dtype != torch.float32 or logits.stride(1) != 1 and experts > 1 or logits.stride(0) < experts and tokens > 1:
+    if logits.dtype is not torch.float32 or logits.stride(1) != 1 and experts > 1 or logits.stride(0) < experts and tokens > 1:
         logits = logits.float().contiguous()
     if bias is not None:
         if bias.shape != (experts,):
             raise ValueError(f"bias must have {experts} values, not the shape {tuple(bias.shape)}")
         bias = bias.float().contiguous()
-    lib, n = _lib.load_decoder(), tokens * top_k
-    ids, weights = torch.empty((tokens, top_k), device=dev, dtype=torch.int32), torch.empty((tokens, top_k), device=dev)
-    order, place = torch.empty(n, device=dev, dtype=torch.int32), torch.empty(n, device=dev, dtype=torch.int32)
-    starts = torch.empty(experts + 1, device=dev, dtype=torch.int32)
+    lib, n, i32 = _lib.load_decoder(), tokens * top_k, torch.int32
+    ids = torch.empty_strided((tokens, top_k), (top_k, 1), device=dev, dtype=i32)
+    weights = torch.empty_strided((tokens, top_k), (top_k, 1), device=dev, dtype=torch.float32)
+    order, place = (torch.empty_strided((n,), (1,), device=dev, dtype=i32) for _ in range(2))
+    starts = torch.empty_strided((experts + 1,), (1,), device=dev, dtype=i32)
     ints = lib.atma_route_scratch_ints(tokens, experts)
     scratch = torch.empty(ints, device=dev, dtype=torch.int32) if ints else None
     _check(lib.atma_route_experts(logits.data_ptr(), logits.stride(0) if tokens > 1 else experts, None if bias is None else bias.data_ptr(), ids.data_ptr(),
@@ -81,8 +82,8 @@ def expert_mlp(x, w_gate_up, w_down, routes, add=None, dtype=torch.bfloat16):
     if tokens == 0:
         return out
     mine = _new_rows(n, width, dev)
-    _check(lib.atma_scatter_rows_fp8(x.values.data_ptr(), _row_stride(x.values), x.scales.data_ptr(), _scale_stride(x.scales), routes.place.data_ptr(), top_k,
-                                     mine.values.data_ptr(), _row_stride(mine.values), mine.scales.data_ptr(), n, tokens, width, _lib.stream_ptr()))
+    _check(lib.atma_scatter_rows_fp8(x.values.data_ptr(), x.row_stride, x.scales.data_ptr(), x.scale_stride, routes.place.data_ptr(), top_k,
+                                     mine.values.data_ptr(), mine.row_stride, mine.scales.data_ptr(), n, tokens, width, _lib.stream_ptr()))
     act = _product(mine, w_gate_up, _new_rows(n, ff, dev), routes.starts, experts)
     y = _product(act, w_down, torch.empty((n, width), device=dev, dtype=dtype), routes.starts, experts)
     _check(lib.atma_combine_experts(y.data_ptr(), routes.place.data_ptr(), routes.weights.data_ptr(), None if add is None else add.data_ptr(), out.data_ptr(),

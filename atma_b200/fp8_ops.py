@@ -24,56 +24,70 @@ def blocks(n):
 
 def _here(*tensors):
     """All of them on the current CUDA device; launches go to its current stream."""
+    here = None
     for t in tensors:
         if t is not None:
-            if not t.is_cuda:
+            at = t.get_device()
+            if at < 0:
                 raise RuntimeError("operations in 8 bits require CUDA tensors (atma_b200 has no CPU path)")
-            if t.device.index != torch._C._cuda_getDevice():
-                raise ValueError(f"a tensor on {t.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+            if here is None:
+                here = torch._C._cuda_getDevice()
+            if at != here:
+                raise ValueError(f"a tensor on {t.device}, the current device is cuda:{here}")
+
+
+def _stride(width):
+    """Bytes between rows that start on 16-byte boundaries."""
+    return width + -width % 16
 
 
 def _storage(shape, width, device):
-    """Rows of ``width`` bytes that start on 16-byte boundaries."""
-    pad = -width % 16
-    return torch.empty((*shape, width + pad), device=device, dtype=E4M3)[..., :width] if pad else torch.empty((*shape, width), device=device, dtype=E4M3)
-
-
-def _on_16_bytes(values):
-    """Whether the rows of (..., rows, width) lie dense behind one another on 16-byte boundaries."""
-    width, step = values.shape[-1], values.stride(-2)
-    if values.stride(-1) != 1 and width > 1 or values.data_ptr() % 16:
-        return False
-    if values.numel() == width:                                                    # one row: its stride is not used
-        return True
-    if step % 16 or step < width:
-        return False
-    for d in range(values.ndim - 3, -1, -1):
-        step *= values.shape[d + 1]
-        if values.shape[d] > 1 and values.stride(d) != step:
-            return False
-    return True
+    """Values whose rows lie dense on 16-byte boundaries."""
+    strides = [_stride(width), 1]
+    for n in reversed(shape[1:]):
+        strides.insert(0, strides[0] * n)
+    return torch.empty_strided((*shape, width), strides, device=device, dtype=E4M3)
 
 
 def _row_stride(values):
-    return values.stride(-2) if values.numel() != values.shape[-1] else -(-values.shape[-1] // 16) * 16
+    """Bytes between the rows of (..., rows, width) if they lie dense behind one another on 16-byte boundaries, else None."""
+    shape, strides = values.shape, values.stride()
+    width = shape[-1]
+    if strides[-1] != 1 and width > 1 or values.data_ptr() % 16:
+        return None
+    if values.numel() == width:                                                    # one row: its stride is not used
+        return _stride(width)
+    step = rs = strides[-2]
+    if step % 16 or step < width:
+        return None
+    for d in range(len(shape) - 3, -1, -1):
+        step *= shape[d + 1]
+        if shape[d] > 1 and strides[d] != step:
+            return None
+    return rs
 
 
 class Fp8Rows:
     """Rows in 8 bits: ``values`` (rows, width) float8_e4m3fn, ``scales`` (rows, blocks) float32.  Rows that do not start on 16-byte
     boundaries and scales that do not lie block by block (stride 1 along the rows) are copied."""
 
-    __slots__ = ("values", "scales")
+    __slots__ = ("values", "scales", "row_stride", "scale_stride")
 
     def __init__(self, values, scales):
-        if values.ndim != 2 or values.dtype != E4M3 or scales.dtype != torch.float32 or scales.shape != (values.shape[0], blocks(values.shape[1])):
+        if values.ndim != 2 or values.dtype is not E4M3 or scales.dtype is not torch.float32 or scales.shape != (values.shape[0], blocks(values.shape[1])):
             raise ValueError("rows in 8 bits are (rows, width) float8_e4m3fn values and (rows, blocks of 128) float32 scales")
-        if scales.device != values.device:
+        if scales.get_device() != values.get_device():
             raise ValueError("values and scales must be on one device")
-        if not _on_16_bytes(values):
+        rs = _row_stride(values)
+        if rs is None:
             values = _storage(values.shape[:1], values.shape[1], values.device).copy_(values)
-        if scales.shape[0] > 1 and scales.stride(0) != 1 or scales.shape[1] > 1 and scales.stride(1) < scales.shape[0]:
-            scales = scales.t().contiguous().t()
-        self.values, self.scales = values, scales
+            rs = _stride(values.shape[1])
+        rows, many = scales.shape
+        along, step = scales.stride()
+        if rows > 1 and along != 1 or many > 1 and step < rows:
+            scales, step = scales.t().contiguous().t(), rows
+        self.values, self.scales, self.row_stride = values, scales, rs
+        self.scale_stride = step if many > 1 and step > rows else rows if rows else 1       # words between neighbouring blocks' scales
 
     @property
     def shape(self):
@@ -88,26 +102,23 @@ class Fp8Rows:
         return self.values.float() * self.scales.repeat_interleave(BLOCK, 1)[:, :self.shape[1]]
 
 
-def _scale_stride(scales):
-    """Words between the scales of neighbouring blocks."""
-    return max(scales.stride(1), scales.shape[0]) if scales.shape[1] > 1 else max(scales.shape[0], 1)
-
-
 class Fp8Weight:
     """A weight in 8 bits: ``values`` (..., N, K) float8_e4m3fn, ``scales`` (..., blocks of N, blocks of K) float32.  Leading dimensions
     hold matrices of one shape: an expert's, or the gate and the up projection of a feed-forward (2, N, K)."""
 
-    __slots__ = ("values", "scales")
+    __slots__ = ("values", "scales", "row_stride")
 
     def __init__(self, values, scales):
-        if values.ndim < 2 or values.dtype != E4M3 or scales.dtype != torch.float32 or \
+        if values.ndim < 2 or values.dtype is not E4M3 or scales.dtype is not torch.float32 or \
                 scales.shape != (*values.shape[:-2], blocks(values.shape[-2]), blocks(values.shape[-1])):
             raise ValueError("a weight in 8 bits is (..., N, K) float8_e4m3fn values and (..., N / 128, K / 128) float32 scales")
-        if scales.device != values.device:
+        if scales.get_device() != values.get_device():
             raise ValueError("values and scales must be on one device")
-        if not _on_16_bytes(values):
+        rs = _row_stride(values)
+        if rs is None:
             values = _storage(values.shape[:-1], values.shape[-1], values.device).copy_(values)
-        self.values, self.scales = values, scales if scales.is_contiguous() else scales.contiguous()
+            rs = _stride(values.shape[-1])
+        self.values, self.scales, self.row_stride = values, scales if scales.is_contiguous() else scales.contiguous(), rs
 
     @classmethod
     def of(cls, weight):
@@ -141,8 +152,10 @@ class Fp8Weight:
 
 
 def _new_rows(rows, width, device):
-    r = Fp8Rows.__new__(Fp8Rows)
-    r.values, r.scales = _storage((rows,), width, device), torch.empty((blocks(width), rows), device=device).t()
+    r, bs = Fp8Rows.__new__(Fp8Rows), rows if rows else 1
+    r.row_stride, r.scale_stride = rs, bs = width + -width % 16, bs
+    r.values = torch.empty_strided((rows, width), (rs, 1), device=device, dtype=E4M3)
+    r.scales = torch.empty_strided((rows, -(-width // BLOCK)), (1, bs), device=device, dtype=torch.float32)
     return r
 
 
@@ -155,7 +168,7 @@ def quantize_rows(x):
         x = x.contiguous()
     n, width = x.shape
     r = _new_rows(n, width, x.device)
-    _check(_lib.load_decoder().atma_quantize_rows(x.data_ptr(), x.stride(0), r.values.data_ptr(), _row_stride(r.values), r.scales.data_ptr(), max(n, 1), n,
+    _check(_lib.load_decoder().atma_quantize_rows(x.data_ptr(), x.stride(0), r.values.data_ptr(), r.row_stride, r.scales.data_ptr(), r.scale_stride, n,
                                                   width, _lib.DTYPE_CODE[x.dtype], _lib.stream_ptr()))
     return r
 
@@ -164,46 +177,44 @@ def residual_norms_fp8(x, y, weights, eps, offset=1.0, out=None, plain=False):
     """``decoder_ops.residual_norms`` with results in 8 bits: x + y (x (rows, width) float32; y in the weights' type, or None) goes to
     ``out`` (None: to x itself); for every weight of ``weights`` (one or two, None = skipped) the normalised row times (offset + weight).
     Returns [(Fp8Rows, None)], and with ``plain`` the last norm in the weights' type beside its rows in 8 bits."""
-    weights = list(weights)
-    given = [w for w in weights if w is not None]
-    _here(x, y, out, *given)
-    if not given or len(weights) > 2:
+    first, second = (*weights, None)[:2] if 0 < len(weights) <= 2 else (None, None)
+    some = first if first is not None else second
+    if some is None:
         raise ValueError("one or two norms")
-    dtype, (n, D) = given[0].dtype, x.shape
-    if x.dtype != torch.float32 or not x.is_contiguous() or D == 0:
+    _here(x, y, out, first, second)
+    dtype, shape = some.dtype, x.shape
+    if x.dtype is not torch.float32 or len(shape) != 2 or shape[1] == 0 or not x.is_contiguous():
         raise ValueError("x must be a contiguous float32 matrix")
-    if dtype not in _TYPES or any(w.dtype != dtype or w.shape != (D,) or not w.is_contiguous() for w in given):
+    n, D = shape
+    if dtype not in _TYPES or any(w is not None and (w.dtype is not dtype or w.shape != (D,) or not w.is_contiguous()) for w in (first, second)):
         raise ValueError(f"weights must have {D} values each and one type, bfloat16 or float32")
-    if y is not None and (y.shape != x.shape or y.dtype != dtype or not y.is_contiguous()):
+    if y is not None and (y.shape != shape or y.dtype is not dtype or not y.is_contiguous()):
         raise ValueError("y must be contiguous, of x's shape and of the weights' type")
-    if out is not None and (out.shape != x.shape or out.dtype != torch.float32 or not out.is_contiguous()):
+    if out is not None and (out.shape != shape or out.dtype is not torch.float32 or not out.is_contiguous()):
         raise ValueError("out must be contiguous, of x's shape and float32")
-    to = out if out is not None else x if y is not None else None
-    rows = [None if w is None else _new_rows(n, D, x.device) for w in weights]
-    h = torch.empty((n, D), device=x.device, dtype=dtype) if plain and weights[-1] is not None else None
-    parts = []
-    for i, (w, r) in enumerate(zip(weights, rows)):
-        parts += (None, None, None, None) if w is None else (w.data_ptr(), r.values.data_ptr(), r.scales.data_ptr(),
-                                                             h.data_ptr() if h is not None and i == len(weights) - 1 else None)
-    if len(weights) == 1:
-        parts += (None, None, None, None)
-    some = next(r for r in rows if r is not None)
+    dev, to, last = x.device, out if out is not None else x if y is not None else None, weights[-1] is not None
+    h = torch.empty_strided((n, D), (D, 1), device=dev, dtype=dtype) if plain and last else None
+    h_ptr, parts, rows = None if h is None else h.data_ptr(), [], []
+    for i, w in enumerate((first, second)):
+        r = None if w is None else _new_rows(n, D, dev)
+        rows.append(r)
+        parts += (None, None, None, None) if r is None else (w.data_ptr(), r.values.data_ptr(), r.scales.data_ptr(), h_ptr if i == len(weights) - 1 else None)
     _check(_lib.load_decoder().atma_residual_norms_fp8(x.data_ptr(), None if y is None else y.data_ptr(), None if to is None else to.data_ptr(), *parts, n, D,
-                                                       _row_stride(some.values), max(n, 1), eps, offset, _lib.DTYPE_CODE[dtype], _lib.stream_ptr()))
-    return [(r, h if i == len(rows) - 1 else None) for i, r in enumerate(rows)]
+                                                       D + -D % 16, n if n else 1, eps, offset, _lib.DTYPE_CODE[dtype], _lib.stream_ptr()))
+    return [(r, h if i == len(weights) - 1 else None) for i, r in enumerate(rows[:len(weights)])]
 
 
 def _product(x, w, out, starts=None, groups=1):
     """x w^T into ``out``: a matrix, or Fp8Rows for the gelu-gated form."""
-    a, gated = _lib.Fp8Args(), isinstance(out, Fp8Rows)
-    a.x, a.x_rs, a.x_scales, a.xs_bs = x.values.data_ptr(), _row_stride(x.values), x.scales.data_ptr(), _scale_stride(x.scales)
-    a.w, a.w_rs, a.w_scales = w.values.data_ptr(), _row_stride(w.values), w.scales.data_ptr()
-    (a.M, n), a.K, a.groups, a.form = out.shape, x.shape[1], groups, int(gated)
-    if gated:
-        a.N, a.out, a.out_rs, a.out_scales, a.os_bs = 2 * n, out.values.data_ptr(), _row_stride(out.values), out.scales.data_ptr(), _scale_stride(out.scales)
+    (m, n), k, v = out.shape, x.values.shape[1], w.values
+    if isinstance(out, Fp8Rows):
+        to = (out.values.data_ptr(), out.row_stride, out.scales.data_ptr(), out.scale_stride)
+        sizes = (m, 2 * n, k, groups, 1, 0)
     else:
-        a.N, a.out, a.out_rs, a.dtype = n, out.data_ptr(), out.stride(0) if out.shape[0] > 1 else n, _lib.DTYPE_CODE[out.dtype]
-    a.starts = None if starts is None else starts.data_ptr()
+        to = (out.data_ptr(), out.stride(0) if m > 1 else n, None, 0)
+        sizes = (m, n, k, groups, 0, _lib.DTYPE_CODE[out.dtype])
+    a = _lib.Fp8Args(x.values.data_ptr(), x.row_stride, x.scales.data_ptr(), x.scale_stride, v.data_ptr(), w.row_stride, w.scales.data_ptr(), *to,
+                     None if starts is None else starts.data_ptr(), *sizes)
     _check(_lib.load_decoder().atma_linear_fp8(ctypes.byref(a), _lib.stream_ptr()))
     return out
 
@@ -211,14 +222,16 @@ def _product(x, w, out, starts=None, groups=1):
 def linear_fp8(x, weight, out=None, dtype=torch.bfloat16):
     """x @ weight.T of rows (rows, K) and a weight (N, K) in 8 bits, in ``dtype`` (bfloat16 or float32) or ``out``'s type: sums in fp32,
     rounded once.  ``out``: (rows, N) with contiguous rows, any row stride."""
-    if not isinstance(x, Fp8Rows) or not isinstance(weight, Fp8Weight) or weight.values.ndim != 2 or weight.shape[1] != x.shape[1] or 0 in weight.shape:
+    if not isinstance(x, Fp8Rows) or not isinstance(weight, Fp8Weight) or weight.values.ndim != 2:
         raise ValueError("linear_fp8 takes Fp8Rows (rows, K) and an Fp8Weight (N, K)")
+    (n, K), (N, columns) = x.values.shape, weight.values.shape
+    if columns != K or N == 0 or K == 0:
+        raise ValueError(f"rows of {K} do not fit a weight ({N}, {columns})")
     _here(x.values, weight.values, out)
-    n, N = x.shape[0], weight.shape[0]
     if out is None:
         if dtype not in _TYPES:
             raise ValueError(f"unsupported dtype {dtype}; expected float32 or bfloat16")
-        out = torch.empty((n, N), device=x.values.device, dtype=dtype)
+        out = torch.empty_strided((n, N), (N, 1), device=x.values.device, dtype=dtype)
     elif out.shape != (n, N) or out.dtype not in _TYPES or out.stride(1) != 1 and N > 1 or out.stride(0) < N and n > 1:
         raise ValueError("out must have the result's shape, contiguous rows and type bfloat16 or float32")
     return _product(x, weight, out)
