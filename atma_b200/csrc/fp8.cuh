@@ -3,9 +3,9 @@
 // The largest value of a block lands on 448, e4m3's largest, so that nothing saturates; the lower bound keeps x / s finite for blocks
 // of zeros and of values that an fp32 quotient by 448 would flush.  A NaN in a block makes its scale a NaN, an infinity an infinity:
 // every result that such a row takes part in is a NaN.
-// The quotient is rounded once, to e4m3.  16-bit values over a largest one of their kind lie on, or nearly on, borders between two
-// e4m3 values in numbers (in one block of seven or so), and a quotient that is rounded to fp32 in between lands on the border itself.
-// So it is rounded to odd: a quotient that is not exact keeps a one in its last place, on the right side of every border.
+// Rows that are given (fp8_four, fp8_one): the quotient is rounded once, to e4m3.  16-bit values over a largest one of their kind lie on, or
+// nearly on, borders between two e4m3 values in numbers (in one block of seven or so), and a quotient that is rounded to fp32 in between
+// lands on the border itself.  Results of fp32 arithmetic (.._times): a product with 1 / s, which is off by as little as they are.
 #pragma once
 
 #include <cuda_fp8.h>
@@ -40,12 +40,19 @@ __device__ __forceinline__ float fp8_quotient(float x, float s, float inv) {
 __device__ __forceinline__ uint32_t fp8_two(float a, float b) {                    // a in the low byte
   return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
+__device__ __forceinline__ uint32_t fp8_four_times(const float (&v)[4], float inv) {
+  return fp8_two(v[0] * inv, v[1] * inv) | fp8_two(v[2] * inv, v[3] * inv) << 16;
+}
+// Where products with a little less and a little more than 1 / s give the same values, the quotients do too.
 __device__ __forceinline__ uint32_t fp8_four(const float (&v)[4], float s) {
   const float inv = 1.0f / s;
+  const uint32_t less = fp8_four_times(v, inv * (1.0f - 0x1p-21f)), more = fp8_four_times(v, inv * (1.0f + 0x1p-21f));
+  if (less == more) return less;
   return fp8_two(fp8_quotient(v[0], s, inv), fp8_quotient(v[1], s, inv)) | fp8_two(fp8_quotient(v[2], s, inv), fp8_quotient(v[3], s, inv)) << 16;
 }
 __device__ __forceinline__ uint8_t fp8_one(float v, float s) {
   return __nv_cvt_float_to_fp8(fp8_quotient(v, s, 1.0f / s), __NV_SATFINITE, __NV_E4M3);
 }
+__device__ __forceinline__ uint8_t fp8_one_times(float v, float inv) { return __nv_cvt_float_to_fp8(v * inv, __NV_SATFINITE, __NV_E4M3); }
 
 }  // namespace atma

@@ -33,19 +33,21 @@ __device__ __forceinline__ void load_block(const T* row, int b, int lane, int wi
     }
   }
 }
-// Stores the block's values and its scale.
-template <bool kVec>
+// Stores the block's values and its scale.  kGiven: the values are an input's, see fp8.cuh.
+template <bool kVec, bool kGiven>
 __device__ __forceinline__ void store_block(uint8_t* row, float* scale, int b, int lane, int width, const float (&v)[4]) {
   const float s = fp8_scale(warp_max_nan(max_nan(max_nan(fabsf(v[0]), fabsf(v[1])), max_nan(fabsf(v[2]), fabsf(v[3])))));
+  const float inv = 1.0f / s;
   if (lane == 0) *scale = s;
   if constexpr (kVec) {
     const int c = b * kFp8Block + 4 * lane;
-    if (c < width) *reinterpret_cast<uint32_t*>(row + c) = fp8_four(v, s);
+    const uint32_t q = kGiven ? fp8_four(v, s) : fp8_four_times(v, inv);
+    if (c < width) *reinterpret_cast<uint32_t*>(row + c) = q;
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int c = b * kFp8Block + lane + 32 * e;
-      if (c < width) row[c] = fp8_one(v[e], s);
+      if (c < width) row[c] = kGiven ? fp8_one(v[e], s) : fp8_one_times(v[e], inv);
     }
   }
 }
@@ -66,7 +68,7 @@ quantize_rows_kernel(const T* x, int64_t x_rs, uint8_t* q, int64_t q_rs, float* 
   for (int i = 0; i < kQuantBlocks; ++i) load_block<T, kVec>(x + row * x_rs, b0 + i, lane, width, v[i]);
 #pragma unroll
   for (int i = 0; i < kQuantBlocks; ++i)
-    if (b0 + i < blocks) store_block<kVec>(q + row * q_rs, scales + (b0 + i) * s_bs + row, b0 + i, lane, width, v[i]);
+    if (b0 + i < blocks) store_block<kVec, true>(q + row * q_rs, scales + (b0 + i) * s_bs + row, b0 + i, lane, width, v[i]);
 }
 
 // ---- the residual stream's norms, in 8 bits ---------------------------------------------------------------
@@ -137,7 +139,7 @@ residual_norms_fp8_kernel(const NormArgs a) {
       load_block<T, true>(static_cast<const T*>(o.w), b, lane, a.D, f);
 #pragma unroll
       for (int e = 0; e < 4; ++e) f[e] = c < a.D ? v[i][e] * rs * (a.offset + f[e]) : 0.f;
-      store_block<true>(o.q + row * a.q_rs, o.scales + b * a.s_bs + row, b, lane, a.D, f);
+      store_block<true, false>(o.q + row * a.q_rs, o.scales + b * a.s_bs + row, b, lane, a.D, f);
       if (o.h != nullptr && c < a.D) {
         Some<T, 4> p;
 #pragma unroll
@@ -192,7 +194,7 @@ residual_norms_fp8_any_kernel(const NormArgs a) {
         f[e] = c < a.D ? v[e] * rs * (a.offset + f[e]) : 0.f;
         if (o.h != nullptr && c < a.D) static_cast<T*>(o.h)[base + c] = from_f32<T>(f[e]);
       }
-      store_block<false>(o.q + row * a.q_rs, o.scales + b * a.s_bs + row, b, lane, a.D, f);
+      store_block<false, false>(o.q + row * a.q_rs, o.scales + b * a.s_bs + row, b, lane, a.D, f);
     }
   }
 }

@@ -148,7 +148,7 @@ int atma_delta_step(const atma_delta_args* args, const void* norm_w, void* out, 
 
 /* ---- rows and weights in 8 bits, experts -------------------------------------------------------------------------
  * A row in 8 bits: e4m3 values and for every block b of 128 channels an fp32 scale, s = max(max |x| / 448, 2^-126),
- * q = e4m3(x / s).  Scales lie block by block: scales[b * s_bs + row].  A weight has a scale for every block of 128 rows
+ * q = e4m3(x / s), the quotient of a given x rounded once.  Scales lie block by block: scales[b * s_bs + row].  A weight has a scale for every block of 128 rows
  * and 128 columns, dense [rows / 128][columns / 128].  Rows of values are q_rs bytes apart. */
 
 /* x (rows, width) to 8 bits. */
