@@ -307,7 +307,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
         s_most[turn][side][32 * quarter + lane] = most;
         if (any_gave_up<32 * kSumWarps>(!ok || *abort)) break;
         const float scale = fp8_scale(max_nan(s_most[turn][0][32 * quarter + lane], s_most[turn][1][32 * quarter + lane]));
-        const float inv = 1.0f / scale;
+        const float inv = fp8_inverse(scale);
         if (row < p.m1) {
           if (side == 0) a.out_scales[(int64_t)(p.n0 / 128) * a.os_bs + row] = scale;
           uint8_t* to = static_cast<uint8_t*>(a.out) + (int64_t)row * a.out_rs + f0;
@@ -558,7 +558,7 @@ linear_fp8_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
           if (c < rows) {
             const float scale = fp8_scale(max_nan(max_nan(s_most[0][c], s_most[1][c]), max_nan(s_most[2][c], s_most[3][c])));
             if (feature == 0) a.out_scales[(int64_t)(p.n0 / 128) * a.os_bs + p.m0 + c] = scale;
-            if (col < a.width) static_cast<uint8_t*>(a.out)[(int64_t)(p.m0 + c) * a.out_rs + col] = fp8_one_times(v[c], 1.0f / scale);
+            if (col < a.width) static_cast<uint8_t*>(a.out)[(int64_t)(p.m0 + c) * a.out_rs + col] = fp8_one_times(v[c], fp8_inverse(scale));
           }
         asm volatile("bar.sync 1, 128;" ::: "memory");       // s_most is read
       } else if (col < a.width) {
@@ -599,7 +599,7 @@ linear_fp8_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
           asm volatile("bar.sync 1, 128;" ::: "memory");
           const float scale = fp8_scale(max_nan(max_nan(s_most[0][c], s_most[1][c]), max_nan(s_most[2][c], s_most[3][c])));
           if (feature == 0) a.out_scales[(int64_t)(p.n0 / 128) * a.os_bs + p.m0 + c] = scale;
-          if (col < a.width) static_cast<uint8_t*>(a.out)[(int64_t)(p.m0 + c) * a.out_rs + col] = fp8_one_times(v[0], 1.0f / scale);
+          if (col < a.width) static_cast<uint8_t*>(a.out)[(int64_t)(p.m0 + c) * a.out_rs + col] = fp8_one_times(v[0], fp8_inverse(scale));
         } else if (col < a.width) {
           static_cast<T*>(a.out)[(int64_t)(p.m0 + c) * a.out_rs + col] = from_f32<T>(v[0]);
         }
