@@ -96,6 +96,19 @@ __device__ __forceinline__ Place place_of(int tile, const int* s_first, const Ar
   return p;
 }
 
+// gelu_tanh(gate) * up of two values each: gate up / (1 + e^-2u), u = sqrt(2 / pi) (z + 0.044715 z^3), by the fast exponential and one
+// reciprocal for both.  The exponent stops at 2^63, where the product of two denominators still fits: results below that are
+// off by 1e-19 of gate * up.  Else off by what gelu_tanh_16 is, 6e-6 at most.
+__device__ __forceinline__ uint64_t gelu_gate_two(uint64_t gate, uint64_t up) {
+  constexpr float kLinear = -2.30220819814f, kCubic = kLinear * 0.044715f;         // -2 sqrt(2 / pi) log2(e)
+  const float2 x = unpack2(mul2(fma2(mul2(gate, gate), pack2(kCubic, kCubic), pack2(kLinear, kLinear)), gate));
+  float e0, e1;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(fminf(x.x, 63.f)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(fminf(x.y, 63.f)));
+  const float a = 1.f + e0, b = 1.f + e1, r = __fdividef(1.f, a * b);
+  return mul2(mul2(gate, up), pack2(r * b, r * a));
+}
+
 // A barrier of kCount threads at which all of them learn whether one has given up: they leave their loops together.
 template <int kCount>
 __device__ __forceinline__ bool any_gave_up(bool mine) {
@@ -153,6 +166,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
   __shared__ float s_most[kGated ? 2 : 1][2][kGated ? 128 : 1];
   __shared__ uint64_t sc_full[kAhead], sc_empty[kAhead];
   __shared__ float s_scale[kAhead][kTogether][kBM + 2];     // of the rows, then of the weight's two blocks
+  __shared__ Place s_place[kAhead];                         // of the tile that a group's blocks belong to
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t rank;
@@ -167,7 +181,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
   if (tid == 32) {
     for (int i = 0; i < kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 2); }
     for (int i = 0; i < 4; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], kSumWarps); }
-    for (int i = 0; i < kAhead; ++i) { mbar_init(&sc_full[i], 32); mbar_init(&sc_empty[i], kSumWarps); }
+    for (int i = 0; i < kAhead; ++i) { mbar_init(&sc_full[i], 33); mbar_init(&sc_empty[i], kSumWarps); }
     s_abort_v = 0;
     fence_barrier_init();
   }
@@ -244,6 +258,10 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
             for (int i = 0; i < kBM; i += 32) copy_word(&s_scale[at][it - i0][i + lane], a.x_scales + it * a.xs_bs + min(row0 + i, a.M - 1));
             if (lane < 2) copy_word(&s_scale[at][it - i0][kBM + lane], ws + it);
           }
+          if (lane == 0) {
+            s_place[at] = p;
+            mbar_arrive(&sc_full[at]);
+          }
           arrive_behind_copies(&sc_full[at]);
         }
       }
@@ -257,8 +275,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
     uint32_t n = 0, g = 0, turn = 0;        // blocks and groups of scales so far
     bool ok = true;
     for (int tile = pair; tile < tiles && ok; tile += pairs, turn ^= 1) {
-      const Place p = place_of(tile, s_first, a, 2 * kBM, kTileN, n_tiles, kBeside);
-      const int row0 = p.m0 + (int)rank * kBM + 32 * quarter, row = row0 + lane;
+      Place p;
       const int c0 = 128 * side;              // gated: 64 of either half of the weight; else a block's
       uint64_t sum[64];
 #pragma unroll
@@ -266,6 +283,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
       for (int i0 = 0; i0 < a.kb && ok; i0 += kTogether, ++g) {
         const uint32_t sc = g % kAhead;
         if (!(ok = mbar_wait_lean(&sc_full[sc], (g / kAhead) & 1, abort))) break;
+        p = s_place[sc];
         const int blocks = min(kTogether, a.kb - i0);
         for (int it = 0; it < blocks; ++it, ++n) {
           const uint32_t buf = n & 1, slot = 2 * buf + side, at = tmem + (uint32_t(32 * quarter) << 16) + slot * kBM;
@@ -293,15 +311,22 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
         __syncwarp();
         if (lane == 0) mbar_arrive(&sc_empty[sc]);
       }
+      const int row0 = p.m0 + (int)rank * kBM + 32 * quarter, row = row0 + lane;
       if constexpr (kGated) {               // whether it goes on is decided by all warps together, below
         const int f0 = p.n0 + 64 * side;
-        float v[64], most = 0.f;
+        float most = 0.f;
 #pragma unroll
-        for (int i = 0; i < 64; i += 2) {
-          const float2 g = unpack2(sum[i / 2]), u = unpack2(sum[32 + i / 2]);
-          v[i] = f0 + i < a.width ? gelu_tanh_16(g.x) * u.x : 0.f;
-          v[i + 1] = f0 + i + 1 < a.width ? gelu_tanh_16(g.y) * u.y : 0.f;
-          most = max_nan(most, max_nan(fabsf(v[i]), fabsf(v[i + 1])));
+        for (int i = 0; i < 32; ++i) sum[i] = gelu_gate_two(sum[i], sum[32 + i]);
+        if (p.n0 + 128 > a.width)           // what is behind the last column is another matrix's
+#pragma unroll
+          for (int i = 0; i < 64; i += 2) {
+            const float2 f = unpack2(sum[i / 2]);
+            sum[i / 2] = pack2(f0 + i < a.width ? f.x : 0.f, f0 + i + 1 < a.width ? f.y : 0.f);
+          }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float2 f = unpack2(sum[i]);
+          most = max_nan(most, max_nan(fabsf(f.x), fabsf(f.y)));
         }
         // a block's 128 columns are two warps': its largest value through shared memory, in turns of two
         s_most[turn][side][32 * quarter + lane] = most;
@@ -316,7 +341,8 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
             uint32_t q[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const float four[4] = {v[i + 4 * j], v[i + 4 * j + 1], v[i + 4 * j + 2], v[i + 4 * j + 3]};
+              const float2 f = unpack2(sum[(i + 4 * j) / 2]), h = unpack2(sum[(i + 4 * j) / 2 + 1]);
+              const float four[4] = {f.x, f.y, h.x, h.y};
               q[j] = fp8_four_times(four, inv);
             }
             if (f0 + i + 16 <= a.width) *reinterpret_cast<uint4*>(to + i) = make_uint4(q[0], q[1], q[2], q[3]);
