@@ -58,6 +58,7 @@ constexpr int kQuantWarps = 8, kQuantBlocks = 4;            // blocks of a row t
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(32 * kQuantWarps)
 quantize_rows_kernel(const T* x, int64_t x_rs, uint8_t* q, int64_t q_rs, float* scales, int64_t s_bs, int64_t pieces, int per_row, int width) {
+  early_start();
   const int64_t piece = (int64_t)blockIdx.x * kQuantWarps + (threadIdx.x >> 5);
   if (piece >= pieces) return;
   const int lane = threadIdx.x & 31;
@@ -204,6 +205,7 @@ residual_norms_fp8_any_kernel(const NormArgs a) {
 __global__ void __launch_bounds__(128)
 scatter_rows_fp8_kernel(const uint8_t* q, int64_t q_rs, const float* scales, int64_t s_bs, const int32_t* place, int copies, uint8_t* to,
                         int64_t to_rs, float* to_scales, int64_t to_bs, int width, int blocks) {
+  early_start();
   const int64_t row = blockIdx.x;
   const uint8_t* from = q + row * q_rs;
   for (int c = threadIdx.x; c < width / 16; c += 128) {
@@ -219,25 +221,39 @@ scatter_rows_fp8_kernel(const uint8_t* q, int64_t q_rs, const float* scales, int
 }
 
 // ---- the weighted sum of a token's results -------------------------------------------------------------------
+// Eight results of a token at a time, all of them asked for before the first is summed: a row is 4 KB, and a token by itself is all latency.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(128)
 combine_experts_kernel(const T* y, const int32_t* place, const float* weights, const T* add, T* out, int copies, int D) {
+  early_start();
+  constexpr int kAtOnce = 8;
   const int64_t row = blockIdx.x;
-  const int c = (blockIdx.y * 128 + threadIdx.x) * VEC;
-  if (c >= D) return;
+  const int c = (blockIdx.y * 128 + threadIdx.x) * VEC, lane = threadIdx.x & 31;
   float v[VEC] = {};
-  if (add != nullptr) {
+  if (add != nullptr && c < D) {
     const Some<T, VEC> p = *reinterpret_cast<const Some<T, VEC>*>(add + row * D + c);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = to_f32(p.e[e]);
   }
-#pragma unroll 4
-  for (int j = 0; j < copies; ++j) {
-    const float w = weights[row * copies + j];
-    const Some<T, VEC> p = *reinterpret_cast<const Some<T, VEC>*>(y + (int64_t)place[row * copies + j] * D + c);
+  for (int j0 = 0; j0 < copies; j0 += kAtOnce) {
+    const bool mine = lane < kAtOnce && j0 + lane < copies;
+    const int at = mine ? place[row * copies + j0 + lane] : 0;
+    const float weight = mine ? weights[row * copies + j0 + lane] : 0.f;
+    Some<T, VEC> p[kAtOnce];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] = fmaf(w, to_f32(p.e[e]), v[e]);
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int64_t from = __shfl_sync(0xffffffffu, at, j);
+      if (j0 + j < copies && c < D) p[j] = *reinterpret_cast<const Some<T, VEC>*>(y + from * D + c);
+    }
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const float w = __shfl_sync(0xffffffffu, weight, j);
+      if (j0 + j < copies && c < D)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = fmaf(w, to_f32(p[j].e[e]), v[e]);
+    }
   }
+  if (c >= D) return;
   Some<T, VEC> p;
 #pragma unroll
   for (int e = 0; e < VEC; ++e) p.e[e] = from_f32<T>(v[e]);
@@ -270,7 +286,7 @@ extern "C" int atma_quantize_rows(const void* x, int64_t x_rs, void* q, int64_t 
   ATMA_FP8_DISPATCH(dtype, T, {
     const bool vec = width % 4 == 0 && x_rs % 4 == 0 && q_rs % 4 == 0 && fits(x, 4 * sizeof(T)) && fits(q, 4);
     auto* kernel = vec ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>;
-    kernel<<<(unsigned)ctas, 32 * kQuantWarps, 0, st>>>((const T*)x, x_rs, (uint8_t*)q, q_rs, scales, s_bs, pieces, per_row, width);
+    launch_early(rows, kernel, (unsigned)ctas, 32 * kQuantWarps, 0, st, (const T*)x, x_rs, (uint8_t*)q, q_rs, scales, s_bs, pieces, per_row, width);
   });
   return launch_status("quantize_rows");
 }
@@ -310,8 +326,8 @@ extern "C" int atma_scatter_rows_fp8(const void* q, int64_t q_rs, const float* s
   ATMA_REQUIRE(q_rs % 16 == 0 && to_rs % 16 == 0 && fits(q, 16) && fits(to, 16) && q_rs >= width && to_rs >= width && s_bs >= rows &&
                    to_bs >= (int64_t)rows * copies,
                "scatter_rows_fp8: rows must start on 16-byte boundaries");
-  scatter_rows_fp8_kernel<<<(unsigned)rows, 128, 0, (cudaStream_t)stream>>>((const uint8_t*)q, q_rs, scales, s_bs, place, copies, (uint8_t*)to, to_rs,
-                                                                           to_scales, to_bs, width, (width + kFp8Block - 1) / kFp8Block);
+  launch_early(rows, scatter_rows_fp8_kernel, (unsigned)rows, 128, 0, (cudaStream_t)stream, (const uint8_t*)q, q_rs, scales, s_bs, place, copies, (uint8_t*)to,
+               to_rs, to_scales, to_bs, width, (width + kFp8Block - 1) / kFp8Block);
   return launch_status("scatter_rows_fp8");
 }
 
@@ -328,7 +344,7 @@ extern "C" int atma_combine_experts(const void* y, const int32_t* place, const f
     const dim3 grid((unsigned)rows, (unsigned)((D + 128 * (vec ? V : 1) - 1) / (128 * (vec ? V : 1))));
     ATMA_REQUIRE(grid.y <= 65535, "combine_experts: rows of %d channels", D);
     auto* kernel = vec ? combine_experts_kernel<T, V> : combine_experts_kernel<T, 1>;
-    kernel<<<grid, 128, 0, st>>>((const T*)y, place, weights, (const T*)add, (T*)out, copies, D);
+    launch_early(rows, kernel, grid, 128, 0, st, (const T*)y, place, weights, (const T*)add, (T*)out, copies, D);
   });
   return launch_status("combine_experts");
 }

@@ -432,15 +432,17 @@ linear_fp8_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
   const int worker = blockIdx.x / ranks, workers = gridDim.x / ranks;
 
-  early_start();
   if (warp == 0) tmem_alloc(&s_tmem, F::kColumns);
-  if (warp == 2) count_tiles(s_first, a, NT);
   if (tid == 32) {
     for (int i = 0; i < F::kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
     for (int i = 0; i < F::kBufs; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 4); }
     s_abort_v = 0;
     fence_barrier_init();
+    prefetch_tensormap(&tm_x);
+    prefetch_tensormap(&tm_w);
   }
+  early_start();                            // nothing in front of it reads or writes what another kernel does
+  if (warp == 2) count_tiles(s_first, a, NT);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -662,12 +664,14 @@ int launch_rows(const CUtensorMap& x, const CUtensorMap& w, const Args& a, cudaS
   int ranks = 1;                            // CTAs that share a tile, four blocks each at least
   if (a.starts == nullptr)
     while (ranks < 8 && 2 * ranks * tiles <= slots && 4 * 2 * ranks <= a.kb) ranks *= 2;
-  cudaLaunchAttribute attrs[1];
+  cudaLaunchAttribute attrs[2];
+  attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;              // see early.cuh
+  attrs[1].val.programmaticStreamSerializationAllowed = 1;
   attrs[0].id = cudaLaunchAttributeClusterDimension;
   attrs[0].val.clusterDim.x = ranks; attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t c = {};
   c.gridDim = dim3((unsigned)(tiles < slots / ranks ? tiles : slots / ranks) * ranks); c.blockDim = dim3(kRowsThreads);
-  c.dynamicSmemBytes = F::kSmem; c.stream = st; c.attrs = attrs; c.numAttrs = 1;
+  c.dynamicSmemBytes = F::kSmem; c.stream = st; c.attrs = attrs; c.numAttrs = 2;
   ATMA_CUDA_OK(cudaLaunchKernelEx(&c, kern, x, w, a));
   return launch_status("linear_fp8 (few rows)");
 }
