@@ -135,7 +135,7 @@ __device__ __forceinline__ void arrive_behind_copies(uint64_t* bar) {           
 constexpr int kStages = 5, kStageBytes = 2 * kPlane;
 constexpr int kSumWarps = 8, kPairThreads = 128 + 32 * kSumWarps;
 constexpr int kChunk = 32;                                  // columns of TMEM that a thread loads at a time
-constexpr int kStaging = 32 * 64;                           // bytes of a warp's 32 rows x 64 bytes of results
+constexpr int kStaging = 32 * 128;                          // bytes of a warp's 32 rows x 128 bytes of results
 constexpr int kPairSmem = kStages * kStageBytes + kSumWarps * kStaging + 1024;
 constexpr int kBeside = 8;
 
@@ -354,12 +354,12 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
         }
       } else {
         if (!ok) break;
-        constexpr int kCols = 64 / sizeof(T), kPer = 16 / sizeof(T);               // columns of a chunk of 64 bytes, of a piece of 16
+        constexpr int kCols = 128 / sizeof(T), kPer = 16 / sizeof(T);              // columns of a chunk of 128 bytes, of a piece of 16
         T* out = static_cast<T*>(a.out);
 #pragma unroll
         for (int chunk = 0; chunk < 128 / kCols; ++chunk) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < 8; ++q) {
             alignas(16) T o[kPer];
 #pragma unroll
             for (int j = 0; j < kPer; j += 2) {
@@ -367,16 +367,18 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
               o[j] = from_f32<T>(f.x);
               o[j + 1] = from_f32<T>(f.y);
             }
-            *reinterpret_cast<uint4*>(s + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)) = *reinterpret_cast<const uint4*>(o);
+            *reinterpret_cast<uint4*>(s + lane * 128 + ((q ^ (lane & 7)) << 4)) = *reinterpret_cast<const uint4*>(o);
           }
           __syncwarp();
+          const int q = lane & 7, col = p.n0 + c0 + chunk * kCols + q * kPer;
+          T* to = out + (int64_t)(row0 + (lane >> 3)) * a.out_rs + col;
+          const bool full = a.vec && col + kPer <= a.width;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {     // eight rows at a time, 64 bytes each
-            const int r = 8 * i + (lane >> 2), q = lane & 3, col = p.n0 + c0 + chunk * kCols + q * kPer;
-            const uint4 v = *reinterpret_cast<const uint4*>(s + r * 64 + ((q ^ (r >> 1 & 3)) << 4));
+          for (int i = 0; i < 8; ++i, to += 4 * a.out_rs) {  // four rows at a time, 128 bytes each
+            const int r = 4 * i + (lane >> 3);
+            const uint4 v = *reinterpret_cast<const uint4*>(s + r * 128 + ((q ^ (r & 7)) << 4));
             if (row0 + r >= p.m1) continue;
-            T* to = out + (int64_t)(row0 + r) * a.out_rs + col;
-            if (a.vec && col + kPer <= a.width) *reinterpret_cast<uint4*>(to) = v;
+            if (full) *reinterpret_cast<uint4*>(to) = v;
             else {
               const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
@@ -396,6 +398,18 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
   tc_fence_after();
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   if (tid == 0 && s_abort_v) atomicExch(&g_linear_fp8_status, 1);
+}
+
+// The place of another CTA of the cluster, and a word of it.
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float load_cluster(uint32_t addr) {
+  float f;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(addr));
+  return f;
 }
 
 // ---- few rows --------------------------------------------------------------------------------------------
@@ -607,29 +621,32 @@ linear_fp8_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
     if (warp >= 2 && worker < tiles) {
       const Place p = place_of(worker, s_first, a, NT, kBM, n_tiles, 1 << 20);
       const int feature = 32 * (warp & 3) + lane, rows = min(NT, p.m1 - p.m0), col = p.n0 + feature;
-      for (int c = rank; c < rows; c += ranks) {
-        float v[kHalves] = {};
+      constexpr int kAtOnce = 4;            // tokens: their loads are under way together
+      for (int c0 = rank; c0 < rows; c0 += kAtOnce * ranks) {
+        float v[kAtOnce][kHalves] = {};
+#pragma unroll 2
+        for (uint32_t o = 0; o < ranks; ++o) {
+          const uint32_t there = in_cta(smem_u32(smem) + feature * 4, o);
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-          const uint32_t mine = smem_u32(smem) + ((h * NT + c) * 128 + feature) * 4;
-          for (uint32_t o = 0; o < ranks; ++o) {
-            uint32_t there;
-            float f;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(mine), "r"(o));
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(there) : "memory");
-            v[h] += f;
-          }
+          for (int i = 0; i < kAtOnce; ++i)
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) v[i][h] += load_cluster(there + (h * NT + min(c0 + i * (int)ranks, NT - 1)) * 512);
         }
-        if constexpr (kGated) {
-          v[0] = col < a.width ? gelu_tanh_16(v[0]) * v[kHalves - 1] : 0.f;
-          const float most = warp_max_nan(fabsf(v[0]));
-          if (lane == 0) s_most[warp & 3][c] = most;
-          asm volatile("bar.sync 1, 128;" ::: "memory");
-          const float scale = fp8_scale(max_nan(max_nan(s_most[0][c], s_most[1][c]), max_nan(s_most[2][c], s_most[3][c])));
-          if (feature == 0) a.out_scales[(int64_t)(p.n0 / 128) * a.os_bs + p.m0 + c] = scale;
-          if (col < a.width) static_cast<uint8_t*>(a.out)[(int64_t)(p.m0 + c) * a.out_rs + col] = fp8_one_times(v[0], fp8_inverse(scale));
-        } else if (col < a.width) {
-          static_cast<T*>(a.out)[(int64_t)(p.m0 + c) * a.out_rs + col] = from_f32<T>(v[0]);
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+          const int c = c0 + i * ranks;
+          if (c >= rows) break;             // the same for all
+          if constexpr (kGated) {
+            const float f = col < a.width ? gelu_tanh_16(v[i][0]) * v[i][kHalves - 1] : 0.f;
+            const float most = warp_max_nan(fabsf(f));
+            if (lane == 0) s_most[warp & 3][c] = most;
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            const float scale = fp8_scale(max_nan(max_nan(s_most[0][c], s_most[1][c]), max_nan(s_most[2][c], s_most[3][c])));
+            if (feature == 0) a.out_scales[(int64_t)(p.n0 / 128) * a.os_bs + p.m0 + c] = scale;
+            if (col < a.width) static_cast<uint8_t*>(a.out)[(int64_t)(p.m0 + c) * a.out_rs + col] = fp8_one_times(f, fp8_inverse(scale));
+          } else if (col < a.width) {
+            static_cast<T*>(a.out)[(int64_t)(p.m0 + c) * a.out_rs + col] = from_f32<T>(v[i][0]);
+          }
         }
       }
     }
