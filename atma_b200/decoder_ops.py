@@ -281,9 +281,12 @@ def _product(x, weight):
     return linear_f32(x, weight, lib=_lib.load_decoder()) if linear_f32_supported(x, weight) else torch.mm(x, weight.t())
 
 
-def linear(x, weight, out=None):
+def linear(x, weight, out=None, dtype=None):
     """x @ weight.T in the activation dtype: the weight-streaming kernel for up to 16 16-bit rows, ``linear_f32`` for
-    fp32 rows in numbers, cuBLAS otherwise."""
+    fp32 rows in numbers, cuBLAS otherwise.  Of rows and a weight in 8 bits: ``fp8_ops.linear_fp8`` in ``dtype``."""
+    if not isinstance(weight, torch.Tensor):
+        from .fp8_ops import linear_fp8
+        return linear_fp8(x, weight, out, dtype)
     from .inference_ops import decode_linear, decode_linear_supported
     if decode_linear_supported(x, weight):
         return decode_linear(x, weight, out=out, lib=_lib.load_decoder())

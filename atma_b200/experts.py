@@ -10,7 +10,7 @@ import torch
 
 from . import _lib
 from .decoder_ops import _check
-from .fp8_ops import Fp8Rows, Fp8Weight, _here, _new_rows, _product, _TYPES
+from .fp8_ops import Fp8Rows, Fp8Weight, _here, _product, _TYPES, empty_rows
 
 MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 512, 64, 64
 
@@ -81,10 +81,10 @@ def expert_mlp(x, w_gate_up, w_down, routes, add=None, dtype=torch.bfloat16):
     out = torch.empty((tokens, width), device=dev, dtype=dtype)
     if tokens == 0:
         return out
-    mine = _new_rows(n, width, dev)
+    mine = empty_rows(n, width, dev)
     _check(lib.atma_scatter_rows_fp8(x.values.data_ptr(), x.row_stride, x.scales.data_ptr(), x.scale_stride, routes.place.data_ptr(), top_k,
                                      mine.values.data_ptr(), mine.row_stride, mine.scales.data_ptr(), n, tokens, width, _lib.stream_ptr()))
-    act = _product(mine, w_gate_up, _new_rows(n, ff, dev), routes.starts, experts)
+    act = _product(mine, w_gate_up, empty_rows(n, ff, dev), routes.starts, experts)
     y = _product(act, w_down, torch.empty((n, width), device=dev, dtype=dtype), routes.starts, experts)
     _check(lib.atma_combine_experts(y.data_ptr(), routes.place.data_ptr(), routes.weights.data_ptr(), None if add is None else add.data_ptr(), out.data_ptr(),
                                     tokens, top_k, width, _lib.DTYPE_CODE[dtype], _lib.stream_ptr()))

@@ -97,6 +97,17 @@ class Fp8Rows:
         """Some of the rows (a slice)."""
         return Fp8Rows(self.values[rows], self.scales[rows])
 
+    def columns(self, start, stop, used=None):
+        """Columns start .. stop - 1, whole blocks, as rows of their own in the same memory; ``used``: only so many of them, the rest of the
+        last block is left."""
+        if start % BLOCK or not 0 <= start < stop <= self.shape[1] or stop % BLOCK and stop != self.shape[1]:
+            raise ValueError(f"columns {start} to {stop} of {self.shape[1]} are not whole blocks of {BLOCK}")
+        if used is not None:
+            if not 0 < used <= stop - start or blocks(used) != blocks(stop - start):
+                raise ValueError(f"{used} columns do not reach the last of the blocks of {stop - start}")
+            stop = start + used
+        return Fp8Rows(self.values[:, start:stop], self.scales[:, start // BLOCK:blocks(stop)])
+
     def wide(self):
         """What the rows stand for, in fp32."""
         return self.values.float() * self.scales.repeat_interleave(BLOCK, 1)[:, :self.shape[1]]
@@ -151,7 +162,8 @@ class Fp8Weight:
         return self.values.float() * self.scales.repeat_interleave(BLOCK, -2)[..., :n, :].repeat_interleave(BLOCK, -1)[..., :k]
 
 
-def _new_rows(rows, width, device):
+def empty_rows(rows, width, device):
+    """Fp8Rows (rows, width) in new memory, not filled."""
     r, bs = Fp8Rows.__new__(Fp8Rows), rows if rows else 1
     r.row_stride, r.scale_stride = rs, bs = width + -width % 16, bs
     r.values = torch.empty_strided((rows, width), (rs, 1), device=device, dtype=E4M3)
@@ -159,15 +171,18 @@ def _new_rows(rows, width, device):
     return r
 
 
-def quantize_rows(x):
-    """Rows (rows, width) of bfloat16 or float32 in 8 bits."""
-    _here(x)
+def quantize_rows(x, out=None):
+    """Rows (rows, width) of bfloat16 or float32 in 8 bits.  ``out``: Fp8Rows of that shape, such as some columns of wider ones (from a
+    multiple of 128 on)."""
+    _here(x, None if out is None else out.values)
     if x.ndim != 2 or x.dtype not in _TYPES or x.shape[1] == 0:
         raise ValueError("quantize_rows takes a (rows, width) matrix of bfloat16 or float32")
+    if out is not None and out.shape != x.shape:
+        raise ValueError(f"out has the shape {tuple(out.shape)}, x {tuple(x.shape)}")
     if x.stride(1) != 1 and x.shape[1] > 1:
         x = x.contiguous()
     n, width = x.shape
-    r = _new_rows(n, width, x.device)
+    r = empty_rows(n, width, x.device) if out is None else out
     _check(_lib.load_decoder().atma_quantize_rows(x.data_ptr(), x.stride(0), r.values.data_ptr(), r.row_stride, r.scales.data_ptr(), r.scale_stride, n,
                                                   width, _lib.DTYPE_CODE[x.dtype], _lib.stream_ptr()))
     return r
@@ -196,7 +211,7 @@ def residual_norms_fp8(x, y, weights, eps, offset=1.0, out=None, plain=False):
     h = torch.empty_strided((n, D), (D, 1), device=dev, dtype=dtype) if plain and last else None
     h_ptr, parts, rows = None if h is None else h.data_ptr(), [], []
     for i, w in enumerate((first, second)):
-        r = None if w is None else _new_rows(n, D, dev)
+        r = None if w is None else empty_rows(n, D, dev)
         rows.append(r)
         parts += (None, None, None, None) if r is None else (w.data_ptr(), r.values.data_ptr(), r.scales.data_ptr(), h_ptr if i == len(weights) - 1 else None)
     _check(_lib.load_decoder().atma_residual_norms_fp8(x.data_ptr(), None if y is None else y.data_ptr(), None if to is None else to.data_ptr(), *parts, n, D,
@@ -237,11 +252,13 @@ def linear_fp8(x, weight, out=None, dtype=torch.bfloat16):
     return _product(x, weight, out)
 
 
-def gelu_gated_linear_fp8(x, weight):
+def gelu_gated_linear_fp8(x, weight, out=None):
     """gelu_tanh(x @ weight[0].T) * (x @ weight[1].T) of rows (rows, K) and a weight (2, N, K) in 8 bits, back in 8 bits: Fp8Rows
-    (rows, N).  Everything between is fp32."""
+    (rows, N), ``out`` as for ``quantize_rows``.  Everything between is fp32."""
     if not isinstance(x, Fp8Rows) or not isinstance(weight, Fp8Weight) or weight.values.ndim != 3 or weight.shape[0] != 2 or \
             weight.shape[2] != x.shape[1] or 0 in weight.shape:
         raise ValueError("gelu_gated_linear_fp8 takes Fp8Rows (rows, K) and an Fp8Weight (2, N, K)")
-    _here(x.values, weight.values)
-    return _product(x, weight, _new_rows(x.shape[0], weight.shape[1], x.values.device))
+    if out is not None and out.shape != (x.shape[0], weight.shape[1]):
+        raise ValueError(f"out has the shape {tuple(out.shape)}, the result {(x.shape[0], weight.shape[1])}")
+    _here(x.values, weight.values, None if out is None else out.values)
+    return _product(x, weight, empty_rows(x.shape[0], weight.shape[1], x.values.device) if out is None else out)

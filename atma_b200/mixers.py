@@ -3,7 +3,8 @@
 A mixer sits between a layer's norm and its output projection: it owns its input projection (one matrix for all of its
 parts), says how many columns it hands to the output projection (``width``), and keeps its per-sequence state in a
 tensor dictionary from ``new_state``.  ``run(h, out, batch, state, carry)`` fills ``out`` (rows, width) for the step's
-rows: decoding sequences (one row each, first) and prompt portions take their own kernels; ``carry`` is a dictionary in
+rows: decoding sequences (one row each, first) and prompt portions take their own kernels; with ``w_in`` in 8 bits (an ``Fp8Weight``) h is rows in
+8 bits too; ``carry`` is a dictionary in
 which the layers of one step leave values for later ones.  All constants are arguments, so a design combines mixers by
 configuration.
 """
@@ -65,6 +66,7 @@ class SoftmaxAttention:
         if rotary is not None and (norms is not None or first_values is not None):
             raise ValueError("rotary positions do not combine with projection norms or value mixing")
         self.w_in = torch.cat([w_q, w_k, w_v] + ([] if w_gate is None else [w_gate])).contiguous()
+        self.dtype, self.device = self.w_in.dtype, self.w_in.device
         self.heads, self.kv_heads, self.maps, self.dim, self.vdim = heads, kv_heads, maps, dim, vdim
         self.scale, self.rotary, self.lam, self.out_scale, self.eps = scale, rotary, lam, out_scale, eps
         self.norms = norms if norms is not None else (None, None, 0.0)
@@ -78,7 +80,7 @@ class SoftmaxAttention:
         return None if self.window is None else (self.window, self.keep_first)
 
     def new_state(self, max_seqs, num_blocks, block_size):
-        dt, dev = self.w_in.dtype, self.w_in.device
+        dt, dev = self.dtype, self.device
         zeros = lambda n: torch.zeros(num_blocks, block_size, self.kv_heads, n, device=dev, dtype=dt)   # finite: masked keys weigh 0
         return {"k": zeros(self.maps * self.dim), "v": zeros(self.vdim)}
 
@@ -98,7 +100,7 @@ class SoftmaxAttention:
         return q.view(-1, self.heads, self.maps, self.dim)
 
     def run(self, h, out, batch, state, carry=None):
-        z = ops.linear(h, self.w_in)
+        z = ops.linear(h, self.w_in, dtype=self.dtype)
         q = self._store(z, batch, state, carry)
         gate = z[:, z.shape[1] - self.width:] if self.gated else None
         kw = dict(scale=self.scale, lam=self.lam, out_scale=self.out_scale, eps=self.eps, window=self.window, keep_first=self.keep_first,
@@ -116,16 +118,17 @@ class GatedDelta:
 
     def __init__(self, w_q, w_k, w_v, w_gate, w_a, w_b, weights, eps):
         self.w_in = torch.cat([w_q, w_k, w_v, w_gate, w_a, w_b]).contiguous()
+        self.dtype, self.device = self.w_in.dtype, self.w_in.device
         self.weights, self.eps = weights, eps
         self.width = weights.heads * weights.vdim
 
     def new_state(self, max_seqs, num_blocks, block_size):
-        w, dev = self.weights, self.w_in.device
-        return {"conv": torch.zeros(max_seqs, w.taps, w.channels, device=dev, dtype=self.w_in.dtype),
+        w, dev = self.weights, self.device
+        return {"conv": torch.zeros(max_seqs, w.taps, w.channels, device=dev, dtype=self.dtype),
                 "state": torch.zeros(max_seqs, w.heads, w.dim, w.vdim, device=dev, dtype=torch.float32)}
 
     def run(self, h, out, batch, state, carry=None):
-        z = ops.linear(h, self.w_in)
+        z = ops.linear(h, self.w_in, dtype=self.dtype)
         for group, call in ((batch.decode, ops.delta_step), (batch.prefill, ops.delta_prefill)):
             if group is not None:
                 r = group.rows

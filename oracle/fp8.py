@@ -124,3 +124,72 @@ def expert_mlp(x, w_gate_up, w_down, ids, weights, err=0.0):
             most[t] += abs(w) * y.abs()
             off[t] += abs(w) * (moved @ w_down[e].abs().t() + err * (q[0].abs() * wide) @ w_down[e].abs().t())
     return out, off, most
+
+
+# ---- a Rizurax layer whose projections are in 8 bits, or whose feed-forward is a mixture of experts ------------------------
+def round_rows(x):
+    """What rows stand for after they have been in 8 bits."""
+    return wide_rows(*quantize(x))
+
+
+def round_weight(w):
+    """What a matrix stands for after it has been in 8 bits with scales by blocks of 128 x 128."""
+    out = torch.zeros_like(w)
+    for i in range(0, w.shape[0], BLOCK):
+        for j in range(0, w.shape[1], BLOCK):
+            cell = w[i:i + BLOCK, j:j + BLOCK]
+            s = (cell.abs().max() / 448).clamp_min(2.0 ** -126).float().double()
+            out[i:i + BLOCK, j:j + BLOCK] = to_e4m3(cell / s) * s
+    return out
+
+
+def rizurax_layer(x, w, i, entry, eps, in_8_bits):
+    from . import rizurax as R
+    p, mix, mlp = f"l{i}.", entry["mixer"], entry.get("mlp")
+    rows, weight = (round_rows, round_weight) if in_8_bits else (lambda t: t, lambda t: t)
+    names = [p + "mix." + n for n in (("q", "k", "v", "g", "a", "b") if entry["type"] == "delta" else ("q", "k", "v"))]
+    parts = weight(torch.cat([w[n] for n in names])).split([w[n].shape[0] for n in names])          # one matrix, whose blocks span its parts
+    mixer = {"delta": R.delta_mixer, "attention": R.attention_mixer}[entry["type"]]
+    size = w[p + "mix.o"].shape[1]
+    inner = {**w, **dict(zip(names, parts)), p + "mix.o": torch.eye(size, dtype=x.dtype)}
+    out = x + rows(mixer(rows(R.rms_norm_centered(x, w[p + "norm1"], eps)), inner, p + "mix.", mix, eps)) @ weight(w[p + "mix.o"]).T
+    if mlp is None:
+        return out
+    h = R.rms_norm_centered(x, w[p + "norm2"], eps)
+    gate, up, down = (w[p + "mlp." + n] for n in ("gate", "up", "down"))
+    if mlp.get("kind", "dense") == "dense":
+        a = R.gelu_tanh(rows(h) @ weight(gate).T) * (rows(h) @ weight(up).T)
+        return out + rows(a) @ weight(down).T
+    ids, weights = route(h @ w[p + "mlp.router"].T, mlp["top_k"], mlp.get("score", "softmax"), w[p + "mlp.router.bias"] if mlp.get("bias") else None,
+                         mlp.get("groups", 1), mlp.get("top_groups") or mlp.get("groups", 1), mlp.get("renormalize", True), mlp.get("scale", 1.0))
+    both = [(round_weight(g), round_weight(u)) for g, u in zip(gate, up)]
+    return out + expert_mlp(round_rows(h), both, [round_weight(d) for d in down], ids, weights)[0]
+
+
+def rizurax_forward(cfg, w, tokens):
+    """Logits (T, vocab) of one sequence."""
+    from . import rizurax as R
+    w = {n: t.double() for n, t in w.items()}
+    eps, x = cfg["norm"]["eps"], R.embed(tokens, w, cfg["embedding"].get("bigram"))
+    for i in R.layer_order(cfg):
+        x = rizurax_layer(x, w, i, cfg["layers"][i], eps, cfg.get("weights") == "e4m3")
+    return R.rms_norm_centered(x, w["final.norm"], eps) @ w["head"].T
+
+
+def rizurax_weights(cfg, seed):
+    """``oracle.rizurax.random_weights`` with the experts' tensors."""
+    from . import rizurax as R
+    plain = {**cfg, "layers": [{**e, "mlp": None if (e.get("mlp") or {}).get("kind") == "experts" else e.get("mlp")} for e in cfg["layers"]]}
+    w, g, D = R.random_weights(plain, seed), torch.Generator().manual_seed(1000 + seed), cfg["width"]
+    put = lambda name, *shape, std=None: w.__setitem__(name, (torch.randn(*shape, generator=g) * (shape[-1] ** -0.5 if std is None else std)).bfloat16().float())
+    for i, e in enumerate(cfg["layers"]):
+        m, p = e.get("mlp") or {}, f"l{i}."
+        if m.get("kind") == "experts":
+            put(p + "norm2", D, std=0.2)
+            put(p + "mlp.router", m["experts"], D)
+            if m.get("bias"):
+                put(p + "mlp.router.bias", m["experts"], std=0.1)
+            put(p + "mlp.gate", m["experts"], m["ff"], D)
+            put(p + "mlp.up", m["experts"], m["ff"], D)
+            put(p + "mlp.down", m["experts"], D, m["ff"])
+    return w

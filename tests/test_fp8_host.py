@@ -184,3 +184,57 @@ def test_register_hand_over_of_the_pair_kernel_fits_the_launch():
     dec, inc = (int(re.search(rf"setmaxnreg\.{w}\.sync\.aligned\.u32 (\d+);", src).group(1)) for w in ("dec", "inc"))
     used = [int(n) for n in re.findall(r"pair_kernel.*?Used (\d+) registers", open(log).read(), re.S)]
     assert len(used) == 3 and all(128 * dec + 256 * inc <= 384 * n for n in used), (dec, inc, used)
+
+
+# ---- models --------------------------------------------------------------------------------------------------------------
+def test_oracle_of_layers_in_8_bits_is_near_the_plain_one():
+    """Roundings to 8 bits are half a step of 2^-4 at most, evenly spread: a projection's result is off by 3.6 %, root mean square; of 32
+    projections one behind another 20 %, as a root of the sum of squares."""
+    from oracle import rizurax as R
+    from tests.fp8_util import CONFIGS_8
+    from tests.rizurax_util import logit_error
+    cfg = CONFIGS_8["dense"]
+    w, t = O.rizurax_weights(cfg, 7), list(range(30))
+    a, b = O.rizurax_forward(cfg, w, t), R.forward(cfg, w, t)[0]
+    e = logit_error(a, b)
+    assert 1e-3 < e.median() and e.pow(2).mean().sqrt() < 0.2
+    plain = {**cfg, "weights": None}
+    assert torch.allclose(O.rizurax_forward(plain, w, t), b, rtol=1e-9, atol=1e-9)
+
+
+def test_models_with_8_bits_and_experts_are_built_and_refused():
+    from atma_b200.fp8_ops import Fp8Weight
+    from atma_b200.rizurax import RizuraxModel
+    from tests.fp8_util import CONFIGS_8, experts
+    for name, cfg in CONFIGS_8.items():
+        w = O.rizurax_weights(cfg, 7)
+        m = RizuraxModel(cfg, w, torch.float32, "cpu")
+        for layer, entry in zip(m.layers, cfg["layers"]):
+            eight = cfg.get("weights") == "e4m3"
+            assert isinstance(layer.w_out, Fp8Weight) == isinstance(layer.mixer.w_in, Fp8Weight) == eight
+            if eight and layer.ff:
+                assert layer.w_out.shape[1] == layer.mixed + layer.ff and layer.mixed % 128 == 0
+                assert not layer.w_out.wide()[:, layer.mixer.width:layer.mixed].any()
+            if layer.experts is not None:
+                assert layer.experts.w_gate_up.shape[1] == 2 and layer.ff == 0
+        assert m.weight_bytes() > 0 and m.new_state(2, 4, 16)
+    cfg = CONFIGS_8["both"]
+    with pytest.raises(ValueError, match="unknown weights"):
+        RizuraxModel({**cfg, "weights": "int4"}, O.rizurax_weights(cfg, 7), torch.float32, "cpu")
+    with pytest.raises(KeyError, match="router"):
+        RizuraxModel(cfg, {n: t for n, t in O.rizurax_weights(cfg, 7).items() if not n.endswith("router")}, torch.float32, "cpu")
+    bad = {**cfg, "layers": [experts(cfg["layers"][0], 15, 3, 128)] + cfg["layers"][1:]}
+    with pytest.raises(ValueError, match="router"):
+        RizuraxModel(bad, O.rizurax_weights(cfg, 7), torch.float32, "cpu")
+
+
+def test_columns_of_rows_in_8_bits():
+    from atma_b200.fp8_ops import E4M3, Fp8Rows
+    r = Fp8Rows(torch.zeros(3, 400, dtype=E4M3), torch.zeros(3, 4))
+    c = r.columns(128, 400)
+    assert c.shape == (3, 272) and c.values.data_ptr() == r.values.data_ptr() + 128 and c.row_stride == r.row_stride
+    assert c.scales.shape == (3, 3) and c.scales.data_ptr() == r.scales.data_ptr() + 4 * 3
+    assert r.columns(0, 256, 200).shape == (3, 200)
+    for a, b, used in ((64, 256, None), (0, 100, None), (0, 401, None), (128, 128, None), (0, 256, 100), (0, 256, 257)):
+        with pytest.raises(ValueError):
+            r.columns(a, b, used)
