@@ -97,6 +97,17 @@ class Fp8Args(Structure):
     ]
 
 
+class ExpertArgs(Structure):
+    """Mirror of atma_expert_args (include/atma_decoder.h)."""
+    _fields_ = [
+        ("x", c_void_p), ("x_rs", c_int64), ("x_scales", c_void_p), ("xs_bs", c_int64),
+        ("w_gate_up", c_void_p), ("w_gate_up_rs", c_int64), ("w_gate_up_scales", c_void_p),
+        ("w_down", c_void_p), ("w_down_rs", c_int64), ("w_down_scales", c_void_p),
+        ("place", c_void_p), ("starts", c_void_p), ("weights", c_void_p), ("add", c_void_p), ("out", c_void_p),
+        ("tokens", c_int), ("copies", c_int), ("experts", c_int), ("width", c_int), ("ff", c_int), ("dtype", c_int),
+    ]
+
+
 _SIGNATURES = {
     "atma_last_error": (c_char_p, []),
     "atma_abi_version": (c_int, []),
@@ -213,6 +224,8 @@ _DECODER_SIGNATURES = {
     "atma_route_scratch_ints": (c_int64, [c_int, c_int]),
     "atma_scatter_rows_fp8": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int,
                                       c_void_p]),
+    "atma_expert_mlp": (c_int, [POINTER(ExpertArgs), c_void_p, c_void_p]),
+    "atma_expert_mlp_scratch_bytes": (c_int64, [c_int] * 5),
     "atma_combine_experts": (c_int, [c_void_p] * 5 + [c_int] * 4 + [c_void_p]),
 }
 _SHARED_SYMBOLS = ("atma_last_error", "atma_decode_linear", "atma_linear_act", "atma_linear_f32", "atma_linear_f32_scratch_bytes")

@@ -25,7 +25,7 @@ LIB = LIBS["b200"]
 SHARED = {"error.cu", "sm100_host.cu", "decode_linear.cu", "delta_blocks.cu", "linear_act.cu", "linear_f32.cu"}
 DECODER = {"decoder_rows.cu", "norm_store.cu", "rotary_store.cu", "softmax_attention.cu", "softmax_prefill_sm100.cu", "softmax_rows_f32.cu",
            "softmax_decode_mma.cu",
-           "delta_rule.cu", "delta_scan_sm100.cu", "fp8_rows.cu", "linear_fp8.cu", "route_experts.cu"}
+           "delta_rule.cu", "delta_scan_sm100.cu", "expert_mlp.cu", "fp8_rows.cu", "linear_fp8.cu", "route_experts.cu"}
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo",

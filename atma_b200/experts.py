@@ -6,11 +6,13 @@
 All launches have shapes that the host knows (tokens x top_k rows), so that a step with experts can be captured in a CUDA graph.
 """
 
+import ctypes
+
 import torch
 
 from . import _lib
 from .decoder_ops import _check
-from .fp8_ops import Fp8Rows, Fp8Weight, _here, _product, _TYPES, empty_rows
+from .fp8_ops import Fp8Rows, Fp8Weight, _here, _new, _stream, _TYPES
 
 MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 512, 64, 64
 
@@ -20,10 +22,23 @@ class Routes:
     token * top_k + choice is a row of the experts' products: order[row] = pair (rows by expert, then by pair), place[pair] = row,
     and expert e's rows are starts[e] .. starts[e + 1] - 1 (all int32)."""
 
-    __slots__ = ("ids", "weights", "order", "place", "starts", "experts")
+    __slots__ = ("ids", "weights", "experts", "_plan")
 
-    def __init__(self, ids, weights, order, place, starts):
-        self.ids, self.weights, self.order, self.place, self.starts, self.experts = ids, weights, order, place, starts, starts.shape[0] - 1
+    def __init__(self, ids, weights, experts, plan):
+        self.ids, self.weights, self.experts, self._plan = ids, weights, experts, plan          # plan: order, place and starts, one behind another
+
+    @property
+    def order(self):
+        return self._plan[:self.ids.numel()]
+
+    @property
+    def place(self):
+        n = self.ids.numel()
+        return self._plan[n:2 * n]
+
+    @property
+    def starts(self):
+        return self._plan[2 * self.ids.numel():]
 
 
 def route_experts(logits, top_k, *, score="softmax", bias=None, groups=1, top_groups=None, renormalize=True, scale=1.0):
@@ -32,7 +47,7 @@ def route_experts(logits, top_k, *, score="softmax", bias=None, groups=1, top_gr
     looked at, those with the largest sum of their two best (None: all).  ``renormalize``: a token's weights are divided by their sum (zero where that is
     zero); ``scale`` multiplies them.  Equal ones: the lower index first.  NaN and -inf count as the least finite logit, inf as the
     largest; a choice is decided as in 64-bit arithmetic."""
-    _here(logits, bias)
+    here = _here(logits, bias)
     if logits.ndim != 2 or not logits.is_floating_point():
         raise ValueError("logits must be a (tokens, experts) matrix")
     (tokens, experts), dev = logits.shape, logits.device
@@ -50,16 +65,17 @@ def route_experts(logits, top_k, *, score="softmax", bias=None, groups=1, top_gr
             raise ValueError(f"bias must have {experts} values, not the shape {tuple(bias.shape)}")
         bias = bias.float().contiguous()
     lib, n, i32 = _lib.load_decoder(), tokens * top_k, torch.int32
-    ids = torch.empty_strided((tokens, top_k), (top_k, 1), device=dev, dtype=i32)
-    weights = torch.empty_strided((tokens, top_k), (top_k, 1), device=dev, dtype=torch.float32)
-    order, place = (torch.empty_strided((n,), (1,), device=dev, dtype=i32) for _ in range(2))
-    starts = torch.empty_strided((experts + 1,), (1,), device=dev, dtype=i32)
-    ints = lib.atma_route_scratch_ints(tokens, experts)
-    scratch = torch.empty(ints, device=dev, dtype=torch.int32) if ints else None
-    _check(lib.atma_route_experts(logits.data_ptr(), logits.stride(0) if tokens > 1 else experts, None if bias is None else bias.data_ptr(), ids.data_ptr(),
-                                  weights.data_ptr(), order.data_ptr(), place.data_ptr(), starts.data_ptr(), None if scratch is None else scratch.data_ptr(),
-                                  tokens, experts, top_k, score == "sigmoid", groups, top_groups, bool(renormalize), scale, _lib.stream_ptr()))
-    return Routes(ids, weights, order, place, starts)
+    ids = _new((tokens, top_k), (top_k, 1), device=dev, dtype=i32)
+    weights = _new((tokens, top_k), (top_k, 1), device=dev, dtype=torch.float32)
+    plan = _new((2 * n + experts + 1,), (1,), device=dev, dtype=i32)
+    ints, at = lib.atma_route_scratch_ints(tokens, experts), plan.data_ptr()
+    scratch = _new((ints,), (1,), device=dev, dtype=i32) if ints else None
+    rc = lib.atma_route_experts(logits.data_ptr(), logits.stride(0) if tokens > 1 else experts, None if bias is None else bias.data_ptr(), ids.data_ptr(),
+                                weights.data_ptr(), at, at + 4 * n, at + 8 * n, None if scratch is None else scratch.data_ptr(), tokens, experts, top_k,
+                                score == "sigmoid", groups, top_groups, bool(renormalize), scale, _stream(here))
+    if rc:
+        _check(rc)
+    return Routes(ids, weights, experts, plan)
 
 
 def expert_mlp(x, w_gate_up, w_down, routes, add=None, dtype=torch.bfloat16):
@@ -69,23 +85,22 @@ def expert_mlp(x, w_gate_up, w_down, routes, add=None, dtype=torch.bfloat16):
     results are in that type too before they are summed, in fp32."""
     if not isinstance(x, Fp8Rows) or not isinstance(w_gate_up, Fp8Weight) or not isinstance(w_down, Fp8Weight) or not isinstance(routes, Routes):
         raise ValueError("expert_mlp takes Fp8Rows, two Fp8Weights and Routes")
-    (tokens, width), experts, top_k = x.shape, routes.experts, routes.ids.shape[1]
-    ff = w_down.shape[-1]
-    if w_gate_up.shape != (experts, 2, ff, width) or w_down.shape != (experts, width, ff) or routes.ids.shape[0] != tokens:
+    (tokens, width), (chosen, top_k), experts = x.values.shape, routes.ids.shape, routes.experts
+    ff = w_down.values.shape[-1]
+    if w_gate_up.values.shape != (experts, 2, ff, width) or w_down.values.shape != (experts, width, ff) or chosen != tokens:
         raise ValueError(f"weights of the shapes {tuple(w_gate_up.shape)} and {tuple(w_down.shape)} do not fit rows {tuple(x.shape)} and "
                          f"{tuple(routes.ids.shape)} choices of {experts} experts")
-    if dtype not in _TYPES or add is not None and (add.shape != x.shape or add.dtype != dtype or not add.is_contiguous()):
+    if dtype not in _TYPES or add is not None and (add.shape != (tokens, width) or add.dtype is not dtype or not add.is_contiguous()):
         raise ValueError("bfloat16 or float32, add contiguous in the same type")
-    _here(x.values, w_gate_up.values, w_down.values, routes.ids, add)
-    lib, n, dev = _lib.load_decoder(), tokens * top_k, x.values.device
-    out = torch.empty((tokens, width), device=dev, dtype=dtype)
-    if tokens == 0:
-        return out
-    mine = empty_rows(n, width, dev)
-    _check(lib.atma_scatter_rows_fp8(x.values.data_ptr(), x.row_stride, x.scales.data_ptr(), x.scale_stride, routes.place.data_ptr(), top_k,
-                                     mine.values.data_ptr(), mine.row_stride, mine.scales.data_ptr(), n, tokens, width, _lib.stream_ptr()))
-    act = _product(mine, w_gate_up, empty_rows(n, ff, dev), routes.starts, experts)
-    y = _product(act, w_down, torch.empty((n, width), device=dev, dtype=dtype), routes.starts, experts)
-    _check(lib.atma_combine_experts(y.data_ptr(), routes.place.data_ptr(), routes.weights.data_ptr(), None if add is None else add.data_ptr(), out.data_ptr(),
-                                    tokens, top_k, width, _lib.DTYPE_CODE[dtype], _lib.stream_ptr()))
+    here, dev = _here(x.values, w_gate_up.values, w_down.values, routes.ids, add), x.values.device
+    lib, code = _lib.load_decoder(), _lib.DTYPE_CODE[dtype]
+    out = _new((tokens, width), (width, 1), device=dev, dtype=dtype)
+    scratch = _new((lib.atma_expert_mlp_scratch_bytes(tokens, top_k, width, ff, code),), (1,), device=dev, dtype=torch.uint8)
+    place = routes._plan.data_ptr() + 4 * tokens * top_k
+    a = _lib.ExpertArgs(x.values.data_ptr(), x.row_stride, x.scales.data_ptr(), x.scale_stride, w_gate_up.values.data_ptr(), w_gate_up.row_stride,
+                        w_gate_up.scales.data_ptr(), w_down.values.data_ptr(), w_down.row_stride, w_down.scales.data_ptr(), place, place + 4 * tokens * top_k,
+                        routes.weights.data_ptr(), None if add is None else add.data_ptr(), out.data_ptr(), tokens, top_k, experts, width, ff, code)
+    rc = lib.atma_expert_mlp(ctypes.byref(a), scratch.data_ptr(), _stream(here))
+    if rc:
+        _check(rc)
     return out

@@ -12,6 +12,8 @@ import torch
 from . import _lib
 from .decoder_ops import _check
 
+_new, _device, _stream = torch.empty_strided, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
 BLOCK = 128                           # channels that share a scale
 TOP, LEAST = 448.0, 2.0 ** -126       # the largest e4m3 value, the smallest scale
 E4M3 = torch.float8_e4m3fn
@@ -23,17 +25,14 @@ def blocks(n):
 
 
 def _here(*tensors):
-    """All of them on the current CUDA device; launches go to its current stream."""
-    here = None
+    """All of them on the current CUDA device (its number), to whose current stream launches go."""
+    here = _device()
     for t in tensors:
-        if t is not None:
-            at = t.get_device()
-            if at < 0:
+        if t is not None and t.get_device() != here:
+            if t.get_device() < 0:
                 raise RuntimeError("operations in 8 bits require CUDA tensors (atma_b200 has no CPU path)")
-            if here is None:
-                here = torch._C._cuda_getDevice()
-            if at != here:
-                raise ValueError(f"a tensor on {t.device}, the current device is cuda:{here}")
+            raise ValueError(f"a tensor on {t.device}, the current device is cuda:{here}")
+    return here
 
 
 def _stride(width):
@@ -74,20 +73,24 @@ class Fp8Rows:
     __slots__ = ("values", "scales", "row_stride", "scale_stride")
 
     def __init__(self, values, scales):
-        if values.ndim != 2 or values.dtype is not E4M3 or scales.dtype is not torch.float32 or scales.shape != (values.shape[0], blocks(values.shape[1])):
+        shape = values.shape
+        if len(shape) != 2 or values.dtype is not E4M3 or scales.dtype is not torch.float32 or scales.shape != (shape[0], -(-shape[1] // BLOCK)):
             raise ValueError("rows in 8 bits are (rows, width) float8_e4m3fn values and (rows, blocks of 128) float32 scales")
         if scales.get_device() != values.get_device():
             raise ValueError("values and scales must be on one device")
-        rs = _row_stride(values)
-        if rs is None:
-            values = _storage(values.shape[:1], values.shape[1], values.device).copy_(values)
-            rs = _stride(values.shape[1])
-        rows, many = scales.shape
+        (rows, width), (step, unit) = shape, values.stride()
+        if rows < 2 or unit != 1 or step < width or step % 16 or values.data_ptr() % 16:
+            step = _row_stride(values)
+            if step is None:
+                values = _storage(shape[:1], width, values.device).copy_(values)
+                step = _stride(width)
+        self.row_stride = step
         along, step = scales.stride()
-        if rows > 1 and along != 1 or many > 1 and step < rows:
+        if width <= BLOCK:                       # one block: its stride is not used
+            step = rows
+        if rows > 1 and along != 1 or step < rows:
             scales, step = scales.t().contiguous().t(), rows
-        self.values, self.scales, self.row_stride = values, scales, rs
-        self.scale_stride = step if many > 1 and step > rows else rows if rows else 1       # words between neighbouring blocks' scales
+        self.values, self.scales, self.scale_stride = values, scales, step if step > 0 else 1      # words between neighbouring blocks' scales
 
     @property
     def shape(self):
@@ -120,8 +123,9 @@ class Fp8Weight:
     __slots__ = ("values", "scales", "row_stride")
 
     def __init__(self, values, scales):
-        if values.ndim < 2 or values.dtype is not E4M3 or scales.dtype is not torch.float32 or \
-                scales.shape != (*values.shape[:-2], blocks(values.shape[-2]), blocks(values.shape[-1])):
+        shape = values.shape
+        if len(shape) < 2 or values.dtype is not E4M3 or scales.dtype is not torch.float32 or \
+                scales.shape != (*shape[:-2], -(-shape[-2] // BLOCK), -(-shape[-1] // BLOCK)):
             raise ValueError("a weight in 8 bits is (..., N, K) float8_e4m3fn values and (..., N / 128, K / 128) float32 scales")
         if scales.get_device() != values.get_device():
             raise ValueError("values and scales must be on one device")
@@ -164,17 +168,17 @@ class Fp8Weight:
 
 def empty_rows(rows, width, device):
     """Fp8Rows (rows, width) in new memory, not filled."""
-    r, bs = Fp8Rows.__new__(Fp8Rows), rows if rows else 1
-    r.row_stride, r.scale_stride = rs, bs = width + -width % 16, bs
-    r.values = torch.empty_strided((rows, width), (rs, 1), device=device, dtype=E4M3)
-    r.scales = torch.empty_strided((rows, -(-width // BLOCK)), (1, bs), device=device, dtype=torch.float32)
+    r = Fp8Rows.__new__(Fp8Rows)
+    r.row_stride, r.scale_stride = rs, bs = width + -width % 16, rows if rows else 1
+    r.values = _new((rows, width), (rs, 1), device=device, dtype=E4M3)
+    r.scales = _new((rows, -(-width // BLOCK)), (1, bs), device=device, dtype=torch.float32)
     return r
 
 
 def quantize_rows(x, out=None):
     """Rows (rows, width) of bfloat16 or float32 in 8 bits.  ``out``: Fp8Rows of that shape, such as some columns of wider ones (from a
     multiple of 128 on)."""
-    _here(x, None if out is None else out.values)
+    here = _here(x, None if out is None else out.values)
     if x.ndim != 2 or x.dtype not in _TYPES or x.shape[1] == 0:
         raise ValueError("quantize_rows takes a (rows, width) matrix of bfloat16 or float32")
     if out is not None and out.shape != x.shape:
@@ -183,8 +187,10 @@ def quantize_rows(x, out=None):
         x = x.contiguous()
     n, width = x.shape
     r = empty_rows(n, width, x.device) if out is None else out
-    _check(_lib.load_decoder().atma_quantize_rows(x.data_ptr(), x.stride(0), r.values.data_ptr(), r.row_stride, r.scales.data_ptr(), r.scale_stride, n,
-                                                  width, _lib.DTYPE_CODE[x.dtype], _lib.stream_ptr()))
+    rc = _lib.load_decoder().atma_quantize_rows(x.data_ptr(), x.stride(0), r.values.data_ptr(), r.row_stride, r.scales.data_ptr(), r.scale_stride, n,
+                                                width, _lib.DTYPE_CODE[x.dtype], _stream(here))
+    if rc:
+        _check(rc)
     return r
 
 
@@ -196,41 +202,55 @@ def residual_norms_fp8(x, y, weights, eps, offset=1.0, out=None, plain=False):
     some = first if first is not None else second
     if some is None:
         raise ValueError("one or two norms")
-    _here(x, y, out, first, second)
+    here = _here(x, y, out, first, second)
     dtype, shape = some.dtype, x.shape
     if x.dtype is not torch.float32 or len(shape) != 2 or shape[1] == 0 or not x.is_contiguous():
         raise ValueError("x must be a contiguous float32 matrix")
     n, D = shape
-    if dtype not in _TYPES or any(w is not None and (w.dtype is not dtype or w.shape != (D,) or not w.is_contiguous()) for w in (first, second)):
-        raise ValueError(f"weights must have {D} values each and one type, bfloat16 or float32")
+    for w in weights:
+        if w is not None and (w.dtype is not dtype or w.shape != (D,) or not w.is_contiguous()) or dtype not in _TYPES:
+            raise ValueError(f"weights must have {D} values each and one type, bfloat16 or float32")
     if y is not None and (y.shape != shape or y.dtype is not dtype or not y.is_contiguous()):
         raise ValueError("y must be contiguous, of x's shape and of the weights' type")
     if out is not None and (out.shape != shape or out.dtype is not torch.float32 or not out.is_contiguous()):
         raise ValueError("out must be contiguous, of x's shape and float32")
-    dev, to, last = x.device, out if out is not None else x if y is not None else None, weights[-1] is not None
-    h = torch.empty_strided((n, D), (D, 1), device=dev, dtype=dtype) if plain and last else None
-    h_ptr, parts, rows = None if h is None else h.data_ptr(), [], []
-    for i, w in enumerate((first, second)):
-        r = None if w is None else empty_rows(n, D, dev)
-        rows.append(r)
-        parts += (None, None, None, None) if r is None else (w.data_ptr(), r.values.data_ptr(), r.scales.data_ptr(), h_ptr if i == len(weights) - 1 else None)
-    _check(_lib.load_decoder().atma_residual_norms_fp8(x.data_ptr(), None if y is None else y.data_ptr(), None if to is None else to.data_ptr(), *parts, n, D,
-                                                       D + -D % 16, n if n else 1, eps, offset, _lib.DTYPE_CODE[dtype], _lib.stream_ptr()))
-    return [(r, h if i == len(weights) - 1 else None) for i, r in enumerate(rows[:len(weights)])]
+    dev, last = x.device, len(weights) - 1
+    to = x if out is None else out
+    h = _new((n, D), (D, 1), device=dev, dtype=dtype) if plain and weights[last] is not None else None
+    parts, results = [], []
+    for i, w in enumerate(weights):
+        if w is None:
+            parts += _NO_NORM
+            results.append((None, None))
+        else:
+            r, beside = empty_rows(n, D, dev), h if i == last else None
+            parts += (w.data_ptr(), r.values.data_ptr(), r.scales.data_ptr(), None if beside is None else beside.data_ptr())
+            results.append((r, beside))
+    if last == 0:
+        parts += _NO_NORM
+    rc = _lib.load_decoder().atma_residual_norms_fp8(x.data_ptr(), None if y is None else y.data_ptr(), None if y is None and out is None else to.data_ptr(),
+                                                     *parts, n, D, D + -D % 16, n if n else 1, eps, offset, _lib.DTYPE_CODE[dtype], _stream(here))
+    if rc:
+        _check(rc)
+    return results
 
 
-def _product(x, w, out, starts=None, groups=1):
+_NO_NORM = (None, None, None, None)
+
+
+def _product(x, w, out, here):
     """x w^T into ``out``: a matrix, or Fp8Rows for the gelu-gated form."""
     (m, n), k, v = out.shape, x.values.shape[1], w.values
     if isinstance(out, Fp8Rows):
         to = (out.values.data_ptr(), out.row_stride, out.scales.data_ptr(), out.scale_stride)
-        sizes = (m, 2 * n, k, groups, 1, 0)
+        sizes = (m, 2 * n, k, 1, 1, 0)
     else:
         to = (out.data_ptr(), out.stride(0) if m > 1 else n, None, 0)
-        sizes = (m, n, k, groups, 0, _lib.DTYPE_CODE[out.dtype])
-    a = _lib.Fp8Args(x.values.data_ptr(), x.row_stride, x.scales.data_ptr(), x.scale_stride, v.data_ptr(), w.row_stride, w.scales.data_ptr(), *to,
-                     None if starts is None else starts.data_ptr(), *sizes)
-    _check(_lib.load_decoder().atma_linear_fp8(ctypes.byref(a), _lib.stream_ptr()))
+        sizes = (m, n, k, 1, 0, _lib.DTYPE_CODE[out.dtype])
+    a = _lib.Fp8Args(x.values.data_ptr(), x.row_stride, x.scales.data_ptr(), x.scale_stride, v.data_ptr(), w.row_stride, w.scales.data_ptr(), *to, None, *sizes)
+    rc = _lib.load_decoder().atma_linear_fp8(ctypes.byref(a), _stream(here))
+    if rc:
+        _check(rc)
     return out
 
 
@@ -242,14 +262,14 @@ def linear_fp8(x, weight, out=None, dtype=torch.bfloat16):
     (n, K), (N, columns) = x.values.shape, weight.values.shape
     if columns != K or N == 0 or K == 0:
         raise ValueError(f"rows of {K} do not fit a weight ({N}, {columns})")
-    _here(x.values, weight.values, out)
+    here = _here(x.values, weight.values, out)
     if out is None:
         if dtype not in _TYPES:
             raise ValueError(f"unsupported dtype {dtype}; expected float32 or bfloat16")
-        out = torch.empty_strided((n, N), (N, 1), device=x.values.device, dtype=dtype)
+        out = _new((n, N), (N, 1), device=x.values.device, dtype=dtype)
     elif out.shape != (n, N) or out.dtype not in _TYPES or out.stride(1) != 1 and N > 1 or out.stride(0) < N and n > 1:
         raise ValueError("out must have the result's shape, contiguous rows and type bfloat16 or float32")
-    return _product(x, weight, out)
+    return _product(x, weight, out, here)
 
 
 def gelu_gated_linear_fp8(x, weight, out=None):
@@ -260,5 +280,5 @@ def gelu_gated_linear_fp8(x, weight, out=None):
         raise ValueError("gelu_gated_linear_fp8 takes Fp8Rows (rows, K) and an Fp8Weight (2, N, K)")
     if out is not None and out.shape != (x.shape[0], weight.shape[1]):
         raise ValueError(f"out has the shape {tuple(out.shape)}, the result {(x.shape[0], weight.shape[1])}")
-    _here(x.values, weight.values, None if out is None else out.values)
-    return _product(x, weight, empty_rows(x.shape[0], weight.shape[1], x.values.device) if out is None else out)
+    here = _here(x.values, weight.values, None if out is None else out.values)
+    return _product(x, weight, empty_rows(x.shape[0], weight.shape[1], x.values.device) if out is None else out, here)

@@ -195,6 +195,22 @@ int atma_scatter_rows_fp8(const void* q, int64_t q_rs, const float* scales, int6
 int atma_combine_experts(const void* y, const int32_t* place, const float* weights, const void* add, void* out, int rows,
                          int copies, int D, int dtype, void* stream);
 
+/* Experts' gelu-gated feed-forwards in 8 bits, weighted and summed: out[t] = add[t] (NULL = 0) + sum over j of weights[t][j]
+ * down_e(gelu_tanh(gate_e x_t) * up_e x_t), e the expert of pair (t, j), for pairs ordered as atma_route_experts does.
+ * x (tokens, width) in 8 bits; w_gate_up [experts][2][ff] rows of width, w_down [experts][width] rows of ff; add and out
+ * (tokens, width) dense in dtype, in which an expert's results are too before they are summed in fp32.
+ * scratch: atma_expert_mlp_scratch_bytes(), 256-byte aligned. */
+typedef struct {
+  const void* x; int64_t x_rs; const float* x_scales; int64_t xs_bs;
+  const void* w_gate_up; int64_t w_gate_up_rs; const float* w_gate_up_scales;
+  const void* w_down; int64_t w_down_rs; const float* w_down_scales;
+  const int32_t* place; const int32_t* starts; const float* weights;
+  const void* add; void* out;
+  int tokens, copies, experts, width, ff, dtype;
+} atma_expert_args;
+int atma_expert_mlp(const atma_expert_args* args, void* scratch, void* stream);
+int64_t atma_expert_mlp_scratch_bytes(int tokens, int copies, int width, int ff, int dtype);
+
 /* Status word of this library's tensor-core kernels (see atma_device_status). */
 int atma_decoder_device_status(int* status);
 

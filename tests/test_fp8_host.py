@@ -91,7 +91,7 @@ def test_refused_arguments(anywhere):
     x, y, w = torch.zeros(4, 256), torch.zeros(4, 256, dtype=torch.bfloat16), torch.zeros(256, dtype=torch.bfloat16)
     r, m = f.Fp8Rows(torch.zeros(4, 256, dtype=f.E4M3), torch.zeros(4, 2)), f.Fp8Weight.of(torch.zeros(8, 256))
     stack = f.Fp8Weight.of(torch.zeros(6, 2, 32, 256)), f.Fp8Weight.of(torch.zeros(6, 256, 32))
-    routes = e.Routes(torch.zeros(4, 2, dtype=torch.int32), torch.zeros(4, 2), None, None, torch.zeros(7, dtype=torch.int32))
+    routes = e.Routes(torch.zeros(4, 2, dtype=torch.int32), torch.zeros(4, 2), 6, torch.zeros(23, dtype=torch.int32))
     z = torch.zeros(4, 12)
     refused = [
         lambda: f.quantize_rows(x.half()), lambda: f.quantize_rows(x[0]), lambda: f.quantize_rows(x[:, :0]),
@@ -152,17 +152,26 @@ def test_the_c_entries_refuse_before_they_launch(lib):
         assert route(**kw) == bad, kw
     assert lib.atma_residual_norms_fp8(p, None, None, p, None, p, None, None, None, None, None, 2, 8, 16, 2, 1e-6, 1.0, 0, None) == bad
     assert lib.atma_combine_experts(p, p, p, None, None, 2, 2, 8, 0, None) == bad
+    mlp = dict(x=4096, x_rs=16, x_scales=4096, xs_bs=2, w_gate_up=4096, w_gate_up_rs=16, w_gate_up_scales=4096, w_down=4096, w_down_rs=16, w_down_scales=4096,
+               place=4096, starts=4096, weights=4096, out=4096, tokens=2, copies=2, experts=3, width=16, ff=16, dtype=1)
+    assert lib.atma_expert_mlp(None, p, None) == bad
+    for change in (dict(dtype=2), dict(tokens=-1), dict(copies=0), dict(width=0), dict(ff=0), dict(place=0), dict(starts=0), dict(weights=0), dict(out=0)):
+        assert lib.atma_expert_mlp(ctypes.byref(_lib.ExpertArgs(**{**mlp, **change})), p, None) == bad, change
+    assert lib.atma_expert_mlp(ctypes.byref(_lib.ExpertArgs(**mlp)), None, None) == bad
+    assert lib.atma_expert_mlp(ctypes.byref(_lib.ExpertArgs(**mlp)), ctypes.c_void_p(4096 + 16), None) == bad
+    assert lib.atma_expert_mlp(ctypes.byref(_lib.ExpertArgs(**{**mlp, "tokens": 0})), None, None) == 0
+    assert lib.atma_expert_mlp_scratch_bytes(3, 2, 20, 130, 1) >= 6 * (32 + 4 + 144 + 8 + 40) and lib.atma_expert_mlp_scratch_bytes(0, 2, 20, 130, 1) == 0
     assert lib.atma_scatter_rows_fp8(p, 16, p, 2, p, 0, p, 16, p, 4, 2, 16, None) == bad
 
 
-def test_fp8_args_layout_matches_the_header():
+def test_argument_layouts_match_the_header():
     from atma_b200 import _lib
-    src = '#include <stdio.h>\n#include "atma_decoder.h"\nint main(void) { printf("%zu\\n", sizeof(atma_fp8_args)); return 0; }\n'
+    src = '#include <stdio.h>\n#include "atma_decoder.h"\nint main(void) { printf("%zu %zu\\n", sizeof(atma_fp8_args), sizeof(atma_expert_args)); return 0; }\n'
     with tempfile.TemporaryDirectory() as d:
         c, exe = os.path.join(d, "s.c"), os.path.join(d, "s")
         open(c, "w").write(textwrap.dedent(src))
         subprocess.check_call(["gcc", "-I", os.path.join(ROOT, "include"), c, "-o", exe])
-        assert ctypes.sizeof(_lib.Fp8Args) == int(subprocess.check_output([exe]))
+        assert [ctypes.sizeof(_lib.Fp8Args), ctypes.sizeof(_lib.ExpertArgs)] == [int(n) for n in subprocess.check_output([exe]).split()]
 
 
 def test_routing_oracle_by_hand():
