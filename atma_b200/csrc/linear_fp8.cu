@@ -50,7 +50,7 @@ struct Args {
   const int32_t* starts;
   int64_t xs_bs, out_rs, os_bs;
   int M, width, K, groups, nb, kb;          // width: columns of results (of one half in the gated form); nb, kb: blocks of width and of K
-  bool vec;                                 // rows of out start on 16-byte boundaries
+  bool vec, sectors;                        // rows of out start on 16-byte and on 32-byte boundaries
 };
 
 // Tiles of every group's rows, `tall` rows each: s_first[g] of them in front of group g's.  Called by a whole warp.
@@ -337,19 +337,29 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
           if (side == 0) a.out_scales[(int64_t)(p.n0 / 128) * a.os_bs + row] = scale;
           uint8_t* to = static_cast<uint8_t*>(a.out) + (int64_t)row * a.out_rs + f0;
 #pragma unroll
-          for (int i = 0; i < 64; i += 16) {
-            uint32_t q[4];
+          for (int i = 0; i < 64; i += 32) {
+            uint32_t q[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 8; ++j) {
               const float2 f = unpack2(sum[(i + 4 * j) / 2]), h = unpack2(sum[(i + 4 * j) / 2 + 1]);
               const float four[4] = {f.x, f.y, h.x, h.y};
               q[j] = fp8_four_times(four, inv);
             }
-            if (f0 + i + 16 <= a.width) *reinterpret_cast<uint4*>(to + i) = make_uint4(q[0], q[1], q[2], q[3]);
-            else
+            if (a.sectors && f0 + i + 32 <= a.width) {       // a whole sector in one go: 330 us with 16 bytes, 316 so (65536 x 2048 x 2048)
+              asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                           ::"l"(to + i), "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3]), "r"(q[4]), "r"(q[5]), "r"(q[6]), "r"(q[7]) : "memory");
+            } else {
 #pragma unroll
-              for (int j = 0; j < 16; ++j)
-                if (f0 + i + j < a.width) to[i + j] = (uint8_t)(q[j >> 2] >> 8 * (j & 3));
+              for (int j = 0; j < 32; j += 16) {
+                if (f0 + i + j + 16 <= a.width) {
+                  *reinterpret_cast<uint4*>(to + i + j) = make_uint4(q[j / 4], q[j / 4 + 1], q[j / 4 + 2], q[j / 4 + 3]);
+                } else {
+#pragma unroll
+                  for (int l = j; l < j + 16; ++l)
+                    if (f0 + i + l < a.width) to[i + l] = (uint8_t)(q[l >> 2] >> 8 * (l & 3));
+                }
+              }
+            }
           }
         }
       } else {
@@ -740,7 +750,8 @@ extern "C" int atma_linear_fp8(const atma_fp8_args* args, void* stream) {
   ATMA_REQUIRE(f.form == 0 || (f.out_scales != nullptr && f.os_bs >= f.M && al16(f.out) && f.out_rs % 16 == 0),
                "linear_fp8: results in 8 bits need scales and rows that start on 16-byte boundaries");
   const Args a{f.x_scales, f.w_scales, f.out, f.out_scales, f.starts, f.xs_bs, f.out_rs, f.os_bs, f.M, width, f.K, f.groups, (width + 127) / 128,
-               (f.K + 127) / 128, al16(f.out) && f.out_rs * (f.dtype == ATMA_F32 ? 4 : 2) % 16 == 0};
+               (f.K + 127) / 128, al16(f.out) && f.out_rs * (f.dtype == ATMA_F32 ? 4 : 2) % 16 == 0,
+               (reinterpret_cast<uintptr_t>(f.out) & 31) == 0 && f.out_rs % 32 == 0};
   cudaStream_t st = (cudaStream_t)stream;
   if (f.form == 1) return launch<float, true>(f, a, st);
   return f.dtype == ATMA_F32 ? launch<float, false>(f, a, st) : launch<__nv_bfloat16, false>(f, a, st);

@@ -27,7 +27,9 @@ namespace {
 
 constexpr int kRouteThreads = 1024, kRouteWarps = kRouteThreads / 32;
 constexpr int kMaxExperts = 512;
-constexpr float kKeyError = 4e-6f;          // twice what fp32 scores and their sum with a bias are off by, relative to |key| + 1
+// Twice what keys are off by, relative to |key| + 1.  Sigmoid: 2 units of e^-z, which s (1 - s) <= 1 / 4 damps, one unit each of 1 + e^-z, its
+// reciprocal and the sum with the bias, 2.5e-7 + 6e-8 |key|.  Softmax: up to 22 roundings of the sum, which all keys share, as well.
+constexpr float kKeyError = 4e-6f, kSigmoidError = 1e-6f;
 
 struct RouteArgs {
   const float* logits; int64_t l_rs;
@@ -141,28 +143,37 @@ __device__ __forceinline__ bool keep_groups(typename Ordered<F>::type (&key)[V],
   return settled;
 }
 
-// The k best of a token: lane j < 32 keeps choice j (and choice j + 32 in the second place).  False where fp32 keys do not settle them.
-template <typename F, int V, bool kExact>
-__device__ __forceinline__ bool choose(const float (&z)[V], int e0, const RouteArgs& a, int (&id)[2], float (&score)[2]) {
+struct Chosen { int id[2]; float score[2]; };                // lane j's choices j and j + 32; id[0] = -1: not settled
+
+__device__ __forceinline__ float logit_of(float f) { return fminf(fmaxf(f, -FLT_MAX), FLT_MAX); }      // a NaN becomes -FLT_MAX
+
+// The k best of a token with keys of type F.  Out of line, and with the logits read again: few tokens come here.
+template <typename F, int V>
+__device__ __noinline__ Chosen choose(const float* row, int e0, const RouteArgs& a) {
   using U = typename Ordered<F>::type;
   const int lane = threadIdx.x & 31;
+  const bool exact = a.bias == nullptr && a.groups == 1;     // keys are the logits
+  float z[V];
   F s[V];
   U key[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) z[v] = e0 + v < a.experts ? logit_of(row[e0 + v]) : -FLT_MAX;
   scores_of<F, V>(z, e0, a.experts, a.sigmoid, s);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int e = e0 + v;
-    F f = kExact ? F(z[v]) : s[v];
-    if (!kExact && a.bias != nullptr && e < a.experts) {
+    F f = exact ? F(z[v]) : s[v];
+    if (a.bias != nullptr && e < a.experts) {
       const float b = a.bias[e];
       f += F(isnan(b) ? -INFINITY : b);
     }
     key[v] = e < a.experts ? ordered(f) : U(0);
   }
   bool settled = true;
-  if (!kExact && a.groups > 1) settled = keep_groups<F, V>(key, e0, a);
+  if (a.groups > 1) settled = keep_groups<F, V>(key, e0, a);
+  Chosen c = {{0, 0}, {0.f, 0.f}};
   U last = 0;
-  const bool check = std::is_same<F, float>::value && !kExact;
+  const bool check = std::is_same<F, float>::value && !exact;
   const int rounds = check && a.k < a.experts ? a.k + 1 : a.k;
   for (int n = 0; n < rounds; ++n) {
     U best = 0;
@@ -182,7 +193,7 @@ __device__ __forceinline__ bool choose(const float (&z)[V], int e0, const RouteA
     const int e = __shfl_sync(0xffffffffu, e0 + where, holder);
     const float got = (float)__shfl_sync(0xffffffffu, at, holder);
     if (lane == (n & 31)) {
-      if (n < 32) { id[0] = e; score[0] = got; } else { id[1] = e; score[1] = got; }
+      if (n < 32) { c.id[0] = e; c.score[0] = got; } else { c.id[1] = e; c.score[1] = got; }
     }
     if (lane == holder) {
 #pragma unroll
@@ -190,13 +201,16 @@ __device__ __forceinline__ bool choose(const float (&z)[V], int e0, const RouteA
         if (v == where) key[v] = 0;
     }
   }
-  return settled;
+  if (!settled) c.id[0] = -1;               // the same for all lanes
+  return c;
 }
 
-template <int V>
-__device__ __noinline__ void choose_in_64(const float (&z)[V], int e0, const RouteArgs& a, int (&id)[2], float (&score)[2]) {
-  if (a.bias == nullptr && a.groups == 1) choose<double, V, true>(z, e0, a, id, score);
-  else choose<double, V, false>(z, e0, a, id, score);
+// 1 / (1 + 2^(-z log2(e))), each step to two units in its last place; zero below z = -87 or so.
+__device__ __forceinline__ float sigmoid_fast(float z) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return r;
 }
 
 // A lane's words in falling order: odd-even merge sort.
@@ -214,6 +228,64 @@ __device__ __forceinline__ void sort_words(uint32_t (&w)[V]) {
         }
 }
 
+// A key in fp64; m: the largest logit, total: the sum of all exp(z - m).
+__device__ __forceinline__ double key_in_64(const float* row, int e, float m, double total, const RouteArgs& a) {
+  const double z = logit_of(row[e]);
+  if (a.bias == nullptr && a.groups == 1) return z;
+  const double s = a.sigmoid ? 1. / (1. + exp(-z)) : exp(z - (double)m) / total;
+  if (a.bias == nullptr) return s;
+  const float b = a.bias[e];
+  return s + (isnan(b) ? -INFINITY : b);
+}
+__device__ __forceinline__ double total_in_64(const float* row, float m, const RouteArgs& a) {
+  double total = 0.;
+  if (!a.sigmoid)
+#pragma unroll 1
+    for (int i = threadIdx.x & 31; i < a.experts; i += 32) total += exp((double)logit_of(row[i]) - (double)m);
+  return warp_add(total);
+}
+
+// Of n taken experts, one a lane, how many have a larger key, in fp64.  Out of line, like the next one: one token in some dozens comes
+// here, and a long way through cold code would hold up its CTA.
+__device__ __noinline__ int rank_in_64(const float* row, int e, int n, float m, const RouteArgs& a) {
+  const double f = key_in_64(row, e, m, total_in_64(row, m, a), a);
+  int above = 0;
+  for (int i = 0; i < n; ++i) {
+    const double g = __shfl_sync(0xffffffffu, f, i);
+    const int h = __shfl_sync(0xffffffffu, e, i);
+    above += g > f || (g == f && h < e);
+  }
+  return (threadIdx.x & 31) < n ? above : 32;
+}
+// Whether this lane's group goes, in fp64 (groups of whole lanes, V experts each).
+template <int V>
+__device__ __noinline__ bool group_goes_in_64(const float* row, int e0, float m, const RouteArgs& a) {
+  const int lanes = a.experts / a.groups / V, mine = (threadIdx.x & 31) & -lanes;
+  const double total = total_in_64(row, m, a);
+  double best = -INFINITY, second = -INFINITY;
+#pragma unroll 2
+  for (int v = 0; v < V; ++v)
+    if (e0 + v < a.experts) {
+      const double f = key_in_64(row, e0 + v, m, total, a);
+      second = fmax(second, fmin(best, f));
+      best = fmax(best, f);
+    }
+#pragma unroll 1
+  for (int o = 1; o < lanes; o <<= 1) {
+    const double b = __shfl_xor_sync(0xffffffffu, best, o), c = __shfl_xor_sync(0xffffffffu, second, o);
+    second = fmax(fmax(second, c), fmin(best, b));
+    best = fmax(best, b);
+  }
+  const double both = V * lanes == 1 ? best : best + second;
+  int above = 0;
+#pragma unroll 1
+  for (int from = 0; from < a.groups * lanes; from += lanes) {
+    const double other = __shfl_sync(0xffffffffu, both, from);
+    above += other > both || (other == both && from < mine);
+  }
+  return above >= a.top_groups;
+}
+
 // The same in fp32 where every lane's experts are of one group (or there are none), a group is 1, 2, 4, .. lanes and k is small.
 //
 // Keys come from instructions that round more; what they are off by stays below kKeyError, since s (1 - s) |z| and |d| exp(-|d|),
@@ -226,7 +298,7 @@ __device__ __forceinline__ bool choose_fast(const float (&z)[V], const float (&b
   constexpr uint32_t kPlace = V <= 8 ? 255 : 511;
   const int lane = threadIdx.x & 31, own = kFull ? V : a.experts - e0;             // the lane's experts, if they are fewer than V
   const bool exact = a.bias == nullptr && a.groups == 1;     // keys are the logits
-  const float width = exact ? 0.f : kKeyError;
+  const float width = exact ? 0.f : a.sigmoid ? kSigmoidError : kKeyError;
   float key[V], m = 0.f, sum = 1.f;
   if (!a.sigmoid) {
     m = z[0];
@@ -245,7 +317,7 @@ __device__ __forceinline__ bool choose_fast(const float (&z)[V], const float (&b
     for (int v = 0; v < V; ++v) key[v] *= r;
   } else if (!exact) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) key[v] = __fdividef(1.f, 1.f + __expf(-z[v]));
+    for (int v = 0; v < V; ++v) key[v] = sigmoid_fast(z[v]);
   }
   if (exact) {
 #pragma unroll
@@ -271,14 +343,16 @@ __device__ __forceinline__ bool choose_fast(const float (&z)[V], const float (&b
     const float both = second == -INFINITY ? best : best + second;
     int above = 0;                          // groups that are better than this lane's
     float nearest = INFINITY;
+#pragma unroll 4
     for (int from = 0; from < a.groups * lanes; from += lanes) {
       const float other = __shfl_sync(0xffffffffu, both, from);
       above += other > both;
       nearest = fminf(nearest, from == mine ? INFINITY : fabsf(other - both));
     }
-    const bool settled = (nearest > 2.f * width * (fabsf(both) + 1.f) && both > -FLT_MAX) || lane >= a.groups * lanes;
-    if (!__all_sync(0xffffffffu, settled)) return false;
+    // two infinities are as near as can be
+    const bool settled = (nearest > 2.f * width * (fabsf(both) + 1.f) && fabsf(both) <= FLT_MAX) || lane >= a.groups * lanes;
     out = above >= a.top_groups;
+    if (!__all_sync(0xffffffffu, settled)) out = group_goes_in_64<V>(row, e0, m, a);
   }
   uint32_t word[V];
 #pragma unroll
@@ -319,31 +393,11 @@ __device__ __forceinline__ bool choose_fast(const float (&z)[V], const float (&b
     } while (true);
   }
   const int e = lane < n ? (int)(kPlace - (taken & kPlace)) : 0;
-  const float x = fminf(fmaxf(row[e], -FLT_MAX), FLT_MAX);
+  const float x = logit_of(row[e]);
   *id = e;
   *rank = lane < n ? lane : 32;
   *score = a.sigmoid ? 1.f / (1.f + expf(-x)) : expf(x - m) / sum;
-  if (near) {                               // the same for all lanes
-    double total = 1., f = x;
-    if (!exact) {
-      if (a.sigmoid) {
-        f = 1. / (1. + exp(-(double)x));
-      } else {
-        total = 0.;
-#pragma unroll 1
-        for (int i = lane; i < a.experts; i += 32) total += exp((double)fminf(fmaxf(row[i], -FLT_MAX), FLT_MAX) - (double)m);
-        f = exp((double)x - (double)m) / warp_add(total);
-      }
-      if (a.bias != nullptr) f += isnan(a.bias[e]) ? -INFINITY : a.bias[e];
-    }
-    int above = 0;
-    for (int i = 0; i < n; ++i) {
-      const double g = __shfl_sync(0xffffffffu, f, i);
-      const int h = __shfl_sync(0xffffffffu, e, i);
-      above += g > f || (g == f && h < e);
-    }
-    if (lane < n) *rank = above;
-  }
+  if (near) *rank = rank_in_64(row, e, n, m, a);             // the same for all lanes
   return true;
 }
 
@@ -415,7 +469,7 @@ __device__ void place_entries(OrderShared& s, const RouteArgs& a, int t0, int t1
 
 template <int V, bool kFull>
 __global__ void __launch_bounds__(kRouteThreads)
-route_experts_kernel(const RouteArgs a) {
+route_experts_kernel(const __grid_constant__ RouteArgs a) {
   early_start();
   __shared__ int32_t s_counts[kMaxExperts];
   extern __shared__ uint8_t s_more[];
@@ -444,16 +498,19 @@ route_experts_kernel(const RouteArgs a) {
     const float* row = a.logits + (int64_t)t * a.l_rs;
     float z[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) z[v] = fminf(fmaxf(next[v], -FLT_MAX), FLT_MAX);   // a NaN becomes -FLT_MAX here
+    for (int v = 0; v < V; ++v) z[v] = logit_of(next[v]);
     if (t + kRouteWarps < t1) bring(t + kRouteWarps);
     // choices of this lane and the places they go to; places behind k are not taken
-    int id[2] = {0, 0}, rank[2] = {lane, lane + 32};
+    int id[2] = {0, 0}, rank[2] = {lane, a.k};
     float score[2] = {0.f, 0.f};
     if (!a.lanes || !choose_fast<V, kFull>(z, bias, e0, a, row, rank, id, score)) {
+      Chosen c = {{-1, 0}, {0.f, 0.f}};
+      if (!a.lanes) c = choose<float, V>(row, e0, a);
+      if (__any_sync(0xffffffffu, c.id[0] < 0)) c = choose<double, V>(row, e0, a);
       rank[0] = lane;
-      if (a.lanes || !choose<float, V, false>(z, e0, a, id, score)) choose_in_64<V>(z, e0, a, id, score);
-    } else {
-      rank[1] = a.k;
+      rank[1] = lane + 32;
+      id[0] = c.id[0]; id[1] = c.id[1];
+      score[0] = c.score[0]; score[1] = c.score[1];
     }
     if (a.renormalize) {
       const float sum = warp_sum((rank[0] < a.k ? score[0] : 0.f) + (rank[1] < a.k ? score[1] : 0.f));
@@ -508,7 +565,7 @@ order_experts_kernel(const RouteArgs a) {
 int route_chunk(int tokens) {
   const int sms = sm_count_of_current_device(), n = (tokens + sms - 1) / sms;
   if (tokens <= 128) return 128;                             // one launch takes less than two
-  return n <= 32 ? 32 : (n + 31) / 32 * 32;
+  return n <= 32 ? 32 : (n + 15) / 16 * 16;
 }
 
 template <int V>

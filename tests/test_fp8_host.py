@@ -193,6 +193,8 @@ def test_register_hand_over_of_the_pair_kernel_fits_the_launch():
     dec, inc = (int(re.search(rf"setmaxnreg\.{w}\.sync\.aligned\.u32 (\d+);", src).group(1)) for w in ("dec", "inc"))
     used = [int(n) for n in re.findall(r"pair_kernel.*?Used (\d+) registers", open(log).read(), re.S)]
     assert len(used) == 3 and all(128 * dec + 256 * inc <= 384 * n for n in used), (dec, inc, used)
+    # sums that do not stay in registers cost half of the rate (232 -> 360 us), and small changes decide whether they do
+    assert re.findall(r"pair_kernel[^\n]*\n.*?(\d+) bytes spill stores", open(log).read(), re.S) == ["0"] * 3
 
 
 # ---- models --------------------------------------------------------------------------------------------------------------

@@ -95,6 +95,25 @@ def test_route_experts_with_experts_that_a_bias_rules_out():
     assert r.ids.tolist() == O.route(x, 3, bias=bias)[0] and all(set(i[:2]) == {0, 1} for i in r.ids.tolist())
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups, top_groups, k", [(8, 3, 5), (4, 2, 9), (16, 7, 6)])
+def test_route_experts_with_groups_that_a_bias_rules_out_or_forces(score, groups, top_groups, k):
+    x, bias = rand((40, 64), 6), rand((64,), 7, 0.1)
+    size = 64 // groups
+    bias[size:3 * size] = -math.inf                          # two whole groups, and one but for a single expert
+    bias[3 * size + 1:4 * size] = -math.inf
+    r = routing().route_experts(x.cuda(), k, score=score, bias=bias.cuda(), groups=groups, top_groups=top_groups)
+    assert r.ids.tolist() == O.route(x, k, score, bias, groups, top_groups)[0]
+    bias[:] = -math.inf                                      # none but two experts of different groups are left
+    bias[5], bias[60] = 0.0, 0.5
+    r = routing().route_experts(x.cuda(), k, score=score, bias=bias.cuda(), groups=groups, top_groups=top_groups)
+    assert r.ids.tolist() == O.route(x, k, score, bias, groups, top_groups)[0]
+    bias[60] = math.inf
+    r = routing().route_experts(x.cuda(), 1, score=score, bias=bias.cuda(), groups=groups, top_groups=top_groups)
+    assert r.ids.flatten().tolist() == [60] * 40
+    check_order(r)
+
+
 def test_route_experts_takes_strided_and_16_bit_logits():
     x = rand((50, 40), 2)
     r = routing().route_experts(x.cuda()[:, 4:36], 3)
