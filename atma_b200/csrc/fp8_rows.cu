@@ -55,9 +55,52 @@ __device__ __forceinline__ void store_block(uint8_t* row, float* scale, int b, i
 // ---- rows to 8 bits ------------------------------------------------------------------------------------
 constexpr int kQuantWarps = 8, kQuantBlocks = 4;            // blocks of a row that a warp has in flight
 
-template <typename T, bool kVec>
+// 16 lanes a block, eight neighbouring channels a lane.
+template <typename T>
 __global__ void __launch_bounds__(32 * kQuantWarps)
 quantize_rows_kernel(const T* x, int64_t x_rs, uint8_t* q, int64_t q_rs, float* scales, int64_t s_bs, int64_t pieces, int per_row, int width) {
+  early_start();
+  const int64_t piece = (int64_t)blockIdx.x * kQuantWarps + (threadIdx.x >> 5);
+  if (piece >= pieces) return;
+  const int lane = threadIdx.x & 31, half = lane >> 4, in = 8 * (lane & 15);
+  const int64_t row = piece / per_row;
+  const int b0 = (int)(piece - row * per_row) * kQuantBlocks + half;
+  float v[kQuantBlocks / 2][8];
+#pragma unroll
+  for (int i = 0; i < kQuantBlocks / 2; ++i) {
+    const int c = (b0 + 2 * i) * kFp8Block + in;
+    Some<T, 4> p[2] = {};
+    if (c < width) {                        // width is a multiple of 8
+      if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(x + row * x_rs + c);
+      } else {
+        p[0] = *reinterpret_cast<const Some<T, 4>*>(x + row * x_rs + c);
+        p[1] = *reinterpret_cast<const Some<T, 4>*>(x + row * x_rs + c + 4);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[i][e] = to_f32(p[e >> 2].e[e & 3]);
+  }
+#pragma unroll
+  for (int i = 0; i < kQuantBlocks / 2; ++i) {
+    float most = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = max_nan(most, fabsf(v[i][e]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+    const float s = fp8_scale(most);
+    const int b = b0 + 2 * i, c = b * kFp8Block + in;
+    if (c >= width) continue;
+    if (in == 0) scales[b * s_bs + row] = s;
+    const float lo[4] = {v[i][0], v[i][1], v[i][2], v[i][3]}, hi[4] = {v[i][4], v[i][5], v[i][6], v[i][7]};
+    *reinterpret_cast<uint2*>(q + row * q_rs + c) = make_uint2(fp8_four(lo, s), fp8_four(hi, s));
+  }
+}
+
+// Any width, stride and address: a warp a block.
+template <typename T>
+__global__ void __launch_bounds__(32 * kQuantWarps)
+quantize_rows_any_kernel(const T* x, int64_t x_rs, uint8_t* q, int64_t q_rs, float* scales, int64_t s_bs, int64_t pieces, int per_row, int width) {
   early_start();
   const int64_t piece = (int64_t)blockIdx.x * kQuantWarps + (threadIdx.x >> 5);
   if (piece >= pieces) return;
@@ -66,10 +109,10 @@ quantize_rows_kernel(const T* x, int64_t x_rs, uint8_t* q, int64_t q_rs, float* 
   const int b0 = (int)(piece - row * per_row) * kQuantBlocks, blocks = (width + kFp8Block - 1) / kFp8Block;
   float v[kQuantBlocks][4];
 #pragma unroll
-  for (int i = 0; i < kQuantBlocks; ++i) load_block<T, kVec>(x + row * x_rs, b0 + i, lane, width, v[i]);
+  for (int i = 0; i < kQuantBlocks; ++i) load_block<T, false>(x + row * x_rs, b0 + i, lane, width, v[i]);
 #pragma unroll
   for (int i = 0; i < kQuantBlocks; ++i)
-    if (b0 + i < blocks) store_block<kVec, true>(q + row * q_rs, scales + (b0 + i) * s_bs + row, b0 + i, lane, width, v[i]);
+    if (b0 + i < blocks) store_block<false, true>(q + row * q_rs, scales + (b0 + i) * s_bs + row, b0 + i, lane, width, v[i]);
 }
 
 // ---- the residual stream's norms, in 8 bits ---------------------------------------------------------------
@@ -284,8 +327,8 @@ extern "C" int atma_quantize_rows(const void* x, int64_t x_rs, void* q, int64_t 
   ATMA_REQUIRE(ctas <= INT32_MAX, "quantize_rows: too many rows");
   cudaStream_t st = (cudaStream_t)stream;
   ATMA_FP8_DISPATCH(dtype, T, {
-    const bool vec = width % 4 == 0 && x_rs % 4 == 0 && q_rs % 4 == 0 && fits(x, 4 * sizeof(T)) && fits(q, 4);
-    auto* kernel = vec ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>;
+    const bool vec = width % 8 == 0 && x_rs % (16 / sizeof(T)) == 0 && q_rs % 8 == 0 && fits(x, 16) && fits(q, 8);
+    auto* kernel = vec ? quantize_rows_kernel<T> : quantize_rows_any_kernel<T>;
     launch_early(rows, kernel, (unsigned)ctas, 32 * kQuantWarps, 0, st, (const T*)x, x_rs, (uint8_t*)q, q_rs, scales, s_bs, pieces, per_row, width);
   });
   return launch_status("quantize_rows");

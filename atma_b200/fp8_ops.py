@@ -129,7 +129,7 @@ class Fp8Weight:
             raise ValueError("a weight in 8 bits is (..., N, K) float8_e4m3fn values and (..., N / 128, K / 128) float32 scales")
         if scales.get_device() != values.get_device():
             raise ValueError("values and scales must be on one device")
-        rs = _row_stride(values)
+        rs = shape[-1] if shape[-1] % 16 == 0 and values.is_contiguous() and values.data_ptr() % 16 == 0 else _row_stride(values)
         if rs is None:
             values = _storage(values.shape[:-1], values.shape[-1], values.device).copy_(values)
             rs = _stride(values.shape[-1])
