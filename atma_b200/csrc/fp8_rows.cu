@@ -1,7 +1,12 @@
-// Row operations around the products in 8 bits: rows to e4m3 with scales, the residual stream's norms with that output,
-// rows copied to the places of their experts and the weighted sum of what comes back.  fp8.cuh says what a block's
-// scale and values are.  A warp owns a block of 128 channels of a row, four of them a lane, so that a block's largest value is a
-// reduction inside of it and nothing is read twice.
+// Row operations around the products in 8 bits: rows to e4m3 with scales, the residual stream's norms with that output, rows copied to the
+// places of their experts and the weighted sum of what comes back.  fp8.cuh says what a block's scale and values are.  Lanes share a block
+// of 128 channels (a warp four each, half a warp eight), so that its largest value is a reduction among them and nothing is read twice.
+//
+// Norms, t = x + y, h = t / sqrt(mean t^2 + eps) (offset + w): a CTA a row, which stays in registers between the sum of squares and the
+// results; scales are written block by block, a word a row, which neighbouring rows' CTAs fill up to sectors in L2.  Bound by HBM and,
+// nearly as much, by instructions (84 % of the issue slots): 32768 x 2048, bf16, two norms, one of them in bf16 too 148 us, 6.4 TB/s; 229 with
+// IEEE quotients and 256 threads a row.  Rows to 8 bits: 8192 x 2048 15.5 us at 1.2 GHz, 3.2 TB/s (21 with four channels a lane).
+// Sum of eight experts' results: 8192 x 8 x 2048 51 us, 6.0 TB/s.
 #include "common.cuh"
 #include "early.cuh"
 #include "fp8.cuh"

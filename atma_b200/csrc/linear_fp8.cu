@@ -9,17 +9,21 @@
 // Many rows (linear_fp8_pair_kernel): two SMs share a tile of 256 rows x 256 columns of results (cta_group::2: each holds its 128 rows of x
 // and half of the weight's rows, so that a block is 32 KB a CTA for 512 clocks of products).  Eight warps a CTA keep 128 sums a thread.
 //   warp 0 TMA, warps 1 and 3 products (of the first CTA, for both; 128 columns each), warp 2 scales, warps 4-11 sums and results.
-// Bound by the way from a product to the next one in its place: they are half a block's (128 columns, two places each), so that its 256
-// clocks and what four warps take to read them (300), plus 570 for the barriers between them, share two blocks' 1024.  8192 x 8192 x 4096
-// (1.25 GHz, the clock that the power leaves): 242 us, 2270 TFLOP/s; the same with whole blocks in two places 250; with a release at cluster
-// scope at every block 605; with scales loaded one block ahead by the warps themselves 13 more; products alone 190, 2880 TFLOP/s.  Tried
-// and slower: 16 warps of 64 sums (276 to 340: more waits than sums), 16 columns of TMEM at a time (248), every warp on both halves
-// (266), the next block's wait and first load in front of the last sums (254).
+// Bound by the way from a product to the next one in its place: places are half a block's (128 columns, two of each half), so that its 256
+// clocks of products and the 300 that four warps take to read them, with 570 for the barriers between them, share two blocks' 1024.  8192 x 8192 x
+// 4096 (1.25 GHz, what the power leaves): 232 to 242 us, 2.3 PFLOP/s, products alone 190.  With whole blocks in two places 250; with a
+// release at cluster scope at every block 605; with scales loaded one block ahead by the warps themselves 13 more.  Tried and slower: 16
+// warps of 64 sums (276 to 340: more waits than sums), 16 columns of TMEM at a time (248), every warp on both halves (266), the next
+// block's wait and first load in front of the last sums (254), results by TMA (no gain, and see below).
+// The sums' 128 registers and two loads of 32 fill what a thread has: a version that spills 20 words takes 360 us.
+// Gated (65536 rows of 64 experts, 2048 x 2048) 300 us, 1.8 PFLOP/s with the gate and the rows behind the experts' ends; 1024 columns, where
+// results leave after every 8 blocks, 175 us, 1.6.
 //
 // Few rows (linear_fp8_rows_kernel): the weight's rows are the tensor core's rows, 128 a tile, and the tokens its columns, 16 to 64, so
-// that a stage is all weight.  Bound by reading that: two CTAs an SM with 100 KB of copies in flight each.  Where a dense product has too few
-// tiles for that, a cluster shares one: every CTA takes its part of the columns, and each then adds up what all of them have for
-// some of the tokens, from their shared memory and in their order.
+// that a stage is all weight.  Bound by reading that: two CTAs an SM with 100 KB of copies in flight each.  128 rows of 64 experts, 2048 x
+// 2048 gated 43 us, 6.2 TB/s; 2048 x 1024 25 us, 5.4.  Where a dense product has too few tiles for that, a cluster shares one: every CTA takes
+// its part of the columns, and each then adds up what all of them have for some of the tokens, from their shared memory and in their
+// order.  8192 x 2048: 4 rows 9.8 us, 64 rows 13.9 (20 with a token's words read one after another), 128 rows 16.4; 200 rows take the other kernel, 16.5.
 //
 // Every mbarrier wait is bounded; on expiry the CTAs free their TMEM, return and leave a status word for the host.
 #include "common.cuh"
@@ -705,7 +709,7 @@ int launch_rows(const CUtensorMap& x, const CUtensorMap& w, const Args& a, cudaS
 
 template <typename T, bool kGated>
 int launch(const atma_fp8_args& f, const Args& a, cudaStream_t st) {
-  // rows of a group, if all have as many
+  // rows of a group, if all have as many; measured above: 128 rows by 64 16.4 us, 200 by the pair kernel 16.5
   const int each = (a.M + a.groups - 1) / a.groups, nt = each <= 16 ? 16 : each <= 32 ? 32 : each <= 128 ? 64 : 0;
   CUtensorMap x, w;
   int rc = make_tmap_8bit_rows(&x, f.x, a.M, f.x_rs, a.K, nt > 0 ? nt : kBM);
