@@ -82,20 +82,22 @@ __device__ __forceinline__ void count_tiles(int* s_first, const Args& a, int tal
 
 struct Place { int group, m0, m1, n0; };    // rows m0 .. of group, whose rows end at m1; columns n0 ..
 
-// Tile `tile` of the groups' n_tiles x (tiles of rows), `beside` tiles of rows beside one another.
-__device__ __forceinline__ Place place_of(int tile, const int* s_first, const Args& a, int tall, int wide, int n_tiles, int beside) {
+// Tile `tile` of the groups' n_tiles x (tiles of rows), kBeside tiles of rows beside one another (0: all of a group's).
+template <int kBeside>
+__device__ __forceinline__ Place place_of(int tile, const int* s_first, const Args& a, int tall, int wide, int n_tiles) {
   int lo = 0, hi = a.groups;                // the last group with s_first * n_tiles <= tile (empty ones are passed over)
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (s_first[mid] * n_tiles <= tile) lo = mid; else hi = mid;
   }
   const int m_tiles = s_first[lo + 1] - s_first[lo], at = tile - s_first[lo] * n_tiles;
-  const int band = at / (beside * n_tiles), in = at - band * beside * n_tiles, high = min(beside, m_tiles - band * beside);
+  const int band = kBeside == 0 ? 0 : at / (kBeside * n_tiles), in = at - band * kBeside * n_tiles;
+  const int high = kBeside == 0 ? m_tiles : min(kBeside, m_tiles - band * kBeside);
   Place p;
   p.group = lo;
   const int first = a.starts == nullptr ? 0 : min(max(a.starts[lo], 0), a.M);
   p.m1 = a.starts == nullptr ? a.M : min(max(a.starts[lo + 1], 0), a.M);
-  p.m0 = first + (band * beside + in % high) * tall;
+  p.m0 = first + (band * kBeside + in % high) * tall;
   p.n0 = in / high * wide;
   return p;
 }
@@ -204,7 +206,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
         uint32_t n = 0;                     // blocks so far, over all tiles
         bool ok = true;
         for (int tile = pair; tile < tiles && ok; tile += pairs) {
-          const Place p = place_of(tile, s_first, a, 2 * kBM, kTileN, n_tiles, kBeside);
+          const Place p = place_of<kBeside>(tile, s_first, a, 2 * kBM, kTileN, n_tiles);
           const int xr = p.m0 + (int)rank * kBM;
           // 64 rows of the weight for either half of the tile's columns
           const int wr = kGated ? (2 * p.group + (int)rank) * a.width + p.n0 : p.group * a.width + p.n0 + (int)rank * 64, next = kGated ? 64 : 128;
@@ -249,7 +251,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
       uint32_t n = 0;
       bool ok = true;
       for (int tile = pair; tile < tiles && ok; tile += pairs) {
-        const Place p = place_of(tile, s_first, a, 2 * kBM, kTileN, n_tiles, kBeside);
+        const Place p = place_of<kBeside>(tile, s_first, a, 2 * kBM, kTileN, n_tiles);
         const int row0 = p.m0 + (int)rank * kBM + lane, block = p.n0 / 128;
         // the blocks of the weight's rows that meet in the tile: two neighbours, or one of either half
         const float* ws = a.w_scales + (kGated ? (int64_t)(2 * p.group + (lane & 1)) * a.nb + block
@@ -485,7 +487,7 @@ linear_fp8_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
       uint32_t n = 0;
       bool ok = true;
       for (int tile = worker; tile < tiles && ok; tile += workers) {
-        const Place p = place_of(tile, s_first, a, NT, kBM, n_tiles, 1 << 20);
+        const Place p = place_of<0>(tile, s_first, a, NT, kBM, n_tiles);
         for (int it = k0; it < k1; ++it, ++n) {
           const uint32_t st = n % F::kStages;
           if (n >= F::kStages && !(ok = mbar_wait(&empty[st], (n / F::kStages - 1) & 1, abort))) break;
@@ -528,7 +530,7 @@ linear_fp8_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
     uint32_t n = 0;
     bool ok = true;
     for (int tile = worker; tile < tiles && ok; tile += workers) {
-      const Place p = place_of(tile, s_first, a, NT, kBM, n_tiles, 1 << 20);
+      const Place p = place_of<0>(tile, s_first, a, NT, kBM, n_tiles);
       const int rows = min(NT, p.m1 - p.m0), col = p.n0 + feature;
       const float* ws = a.w_scales + ((int64_t)kHalves * p.group * a.nb + p.n0 / 128) * a.kb;
       const float* us = ws + (kGated ? (int64_t)a.nb * a.kb : 0);
@@ -633,7 +635,7 @@ linear_fp8_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
     __syncthreads();
     cluster_sync();
     if (warp >= 2 && worker < tiles) {
-      const Place p = place_of(worker, s_first, a, NT, kBM, n_tiles, 1 << 20);
+      const Place p = place_of<0>(worker, s_first, a, NT, kBM, n_tiles);
       const int feature = 32 * (warp & 3) + lane, rows = min(NT, p.m1 - p.m0), col = p.n0 + feature;
       constexpr int kAtOnce = 4;            // tokens: their loads are under way together
       for (int c0 = rank; c0 < rows; c0 += kAtOnce * ranks) {

@@ -11,6 +11,7 @@ import torch
 
 from . import _lib
 from .decoder_ops import _check
+from .inference_ops import _overlap
 
 _new, _device, _stream = torch.empty_strided, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
@@ -33,6 +34,13 @@ def _here(*tensors):
                 raise RuntimeError("operations in 8 bits require CUDA tensors (atma_b200 has no CPU path)")
             raise ValueError(f"a tensor on {t.device}, the current device is cuda:{here}")
     return here
+
+
+def _apart(out, *inputs):
+    """Refuses results over what is read: other CTAs read on while the first ones write."""
+    for t in inputs:
+        if t is not None and _overlap(out, t):
+            raise ValueError("results must not overlap what is read")
 
 
 def _stride(width):
@@ -181,8 +189,10 @@ def quantize_rows(x, out=None):
     here = _here(x, None if out is None else out.values)
     if x.ndim != 2 or x.dtype not in _TYPES or x.shape[1] == 0:
         raise ValueError("quantize_rows takes a (rows, width) matrix of bfloat16 or float32")
-    if out is not None and out.shape != x.shape:
-        raise ValueError(f"out has the shape {tuple(out.shape)}, x {tuple(x.shape)}")
+    if out is not None:
+        if out.shape != x.shape:
+            raise ValueError(f"out has the shape {tuple(out.shape)}, x {tuple(x.shape)}")
+        _apart(out.values, x), _apart(out.scales, x)
     if x.stride(1) != 1 and x.shape[1] > 1:
         x = x.contiguous()
     n, width = x.shape
@@ -212,8 +222,12 @@ def residual_norms_fp8(x, y, weights, eps, offset=1.0, out=None, plain=False):
             raise ValueError(f"weights must have {D} values each and one type, bfloat16 or float32")
     if y is not None and (y.shape != shape or y.dtype is not dtype or not y.is_contiguous()):
         raise ValueError("y must be contiguous, of x's shape and of the weights' type")
-    if out is not None and (out.shape != shape or out.dtype is not torch.float32 or not out.is_contiguous()):
-        raise ValueError("out must be contiguous, of x's shape and float32")
+    if out is not None:
+        if out.shape != shape or out.dtype is not torch.float32 or not out.is_contiguous():
+            raise ValueError("out must be contiguous, of x's shape and float32")
+        at, nbytes = out.data_ptr(), 4 * n * D
+        if at != x.data_ptr() and abs(at - x.data_ptr()) < nbytes or y is not None and -n * D * y.element_size() < y.data_ptr() - at < nbytes:
+            raise ValueError("out may be x, and must not overlap x or y otherwise")
     dev, last = x.device, len(weights) - 1
     to = x if out is None else out
     h = _new((n, D), (D, 1), device=dev, dtype=dtype) if plain and weights[last] is not None else None
@@ -267,8 +281,10 @@ def linear_fp8(x, weight, out=None, dtype=torch.bfloat16):
         if dtype not in _TYPES:
             raise ValueError(f"unsupported dtype {dtype}; expected float32 or bfloat16")
         out = _new((n, N), (N, 1), device=x.values.device, dtype=dtype)
-    elif out.shape != (n, N) or out.dtype not in _TYPES or out.stride(1) != 1 and N > 1 or out.stride(0) < N and n > 1:
-        raise ValueError("out must have the result's shape, contiguous rows and type bfloat16 or float32")
+    else:
+        if out.shape != (n, N) or out.dtype not in _TYPES or out.stride(1) != 1 and N > 1 or out.stride(0) < N and n > 1:
+            raise ValueError("out must have the result's shape, contiguous rows and type bfloat16 or float32")
+        _apart(out, x.values, x.scales, weight.values, weight.scales)
     return _product(x, weight, out, here)
 
 
@@ -278,7 +294,10 @@ def gelu_gated_linear_fp8(x, weight, out=None):
     if not isinstance(x, Fp8Rows) or not isinstance(weight, Fp8Weight) or weight.values.ndim != 3 or weight.shape[0] != 2 or \
             weight.shape[2] != x.shape[1] or 0 in weight.shape:
         raise ValueError("gelu_gated_linear_fp8 takes Fp8Rows (rows, K) and an Fp8Weight (2, N, K)")
-    if out is not None and out.shape != (x.shape[0], weight.shape[1]):
-        raise ValueError(f"out has the shape {tuple(out.shape)}, the result {(x.shape[0], weight.shape[1])}")
     here = _here(x.values, weight.values, None if out is None else out.values)
+    if out is not None:
+        if out.shape != (x.shape[0], weight.shape[1]):
+            raise ValueError(f"out has the shape {tuple(out.shape)}, the result {(x.shape[0], weight.shape[1])}")
+        for t in (out.values, out.scales):
+            _apart(t, x.values, x.scales, weight.values, weight.scales)
     return _product(x, weight, empty_rows(x.shape[0], weight.shape[1], x.values.device) if out is None else out, here)

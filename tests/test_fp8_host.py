@@ -113,6 +113,18 @@ def test_refused_arguments(anywhere):
         lambda: e.expert_mlp(r, *stack, routes, dtype=torch.float16), lambda: e.expert_mlp(r, *stack, routes, add=x),
         lambda: e.expert_mlp(r, *stack, None),
     ]
+    # results over what is read
+    big, gate = torch.zeros(4, 512), f.Fp8Weight.of(torch.zeros(2, 256, 256))
+    memory = torch.zeros(8, 256, dtype=f.E4M3)
+    over = f.Fp8Rows(memory[:4], torch.zeros(2, 4).t())
+    refused += [
+        lambda: f.residual_norms_fp8(big.view(-1)[:1024].view(4, 256), None, [w], 1e-6, out=big.view(-1)[256:1280].view(4, 256)),
+        lambda: f.residual_norms_fp8(x, y, [w], 1e-6, out=torch.as_strided(y.view(torch.float32), (2, 256), (256, 1)).expand(2, 256)),
+        lambda: f.gelu_gated_linear_fp8(over, gate, out=over), lambda: f.gelu_gated_linear_fp8(over, gate, out=f.Fp8Rows(memory[2:6], torch.zeros(2, 4).t())),
+        lambda: f.gelu_gated_linear_fp8(over, gate, out=f.Fp8Rows(memory[4:], over.scales)), lambda: f.gelu_gated_linear_fp8(over, gate, out=over.columns(0, 128)),
+        lambda: f.linear_fp8(over, m, out=memory.view(torch.bfloat16)[:4, :8]), lambda: f.quantize_rows(memory.view(torch.float32)[:4, :64], out=over.columns(0, 128)),
+        lambda: f.quantize_rows(memory.view(torch.bfloat16).view(-1)[:1024].view(4, 256), out=over),
+    ]
     for i, call in enumerate(refused):
         with pytest.raises(ValueError):
             call()

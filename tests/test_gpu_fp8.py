@@ -156,7 +156,8 @@ def product_bound(x, w, dtype):
 
 SHAPES = [(1, 1, 1), (1, 16, 16), (2, 3, 130), (1, 2048, 1024), (16, 300, 777), (17, 64, 128), (33, 129, 127), (64, 1000, 256), (65, 40, 2000), (127, 128, 384),
           (128, 256, 128), (129, 257, 144), (200, 513, 640), (255, 130, 1152), (257, 384, 512), (300, 1000, 1304), (513, 520, 260), (1000, 260, 900),
-          (2600, 2000, 200), (40, 40000, 128)]                            # more tiles than there are CTAs
+          (2600, 2000, 200), (40, 40000, 128),                            # more tiles than there are CTAs
+          (3, 300000, 16), (130, 270000, 16)]                             # vocabularies: tiles of columns in thousands
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
