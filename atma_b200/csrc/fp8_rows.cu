@@ -334,7 +334,7 @@ extern "C" int atma_quantize_rows(const void* x, int64_t x_rs, void* q, int64_t 
   ATMA_FP8_DISPATCH(dtype, T, {
     const bool vec = width % 8 == 0 && x_rs % (16 / sizeof(T)) == 0 && q_rs % 8 == 0 && fits(x, 16) && fits(q, 8);
     auto* kernel = vec ? quantize_rows_kernel<T> : quantize_rows_any_kernel<T>;
-    launch_early(rows, kernel, (unsigned)ctas, 32 * kQuantWarps, 0, st, (const T*)x, x_rs, (uint8_t*)q, q_rs, scales, s_bs, pieces, per_row, width);
+    launch_early(0, kernel, (unsigned)ctas, 32 * kQuantWarps, 0, st, (const T*)x, x_rs, (uint8_t*)q, q_rs, scales, s_bs, pieces, per_row, width);
   });
   return launch_status("quantize_rows");
 }
@@ -374,7 +374,7 @@ extern "C" int atma_scatter_rows_fp8(const void* q, int64_t q_rs, const float* s
   ATMA_REQUIRE(q_rs % 16 == 0 && to_rs % 16 == 0 && fits(q, 16) && fits(to, 16) && q_rs >= width && to_rs >= width && s_bs >= rows &&
                    to_bs >= (int64_t)rows * copies,
                "scatter_rows_fp8: rows must start on 16-byte boundaries");
-  launch_early(rows, scatter_rows_fp8_kernel, (unsigned)rows, 128, 0, (cudaStream_t)stream, (const uint8_t*)q, q_rs, scales, s_bs, place, copies, (uint8_t*)to,
+  launch_early(0, scatter_rows_fp8_kernel, (unsigned)rows, 128, 0, (cudaStream_t)stream, (const uint8_t*)q, q_rs, scales, s_bs, place, copies, (uint8_t*)to,
                to_rs, to_scales, to_bs, width, (width + kFp8Block - 1) / kFp8Block);
   return launch_status("scatter_rows_fp8");
 }
@@ -392,7 +392,7 @@ extern "C" int atma_combine_experts(const void* y, const int32_t* place, const f
     const dim3 grid((unsigned)rows, (unsigned)((D + 128 * (vec ? V : 1) - 1) / (128 * (vec ? V : 1))));
     ATMA_REQUIRE(grid.y <= 65535, "combine_experts: rows of %d channels", D);
     auto* kernel = vec ? combine_experts_kernel<T, V> : combine_experts_kernel<T, 1>;
-    launch_early(rows, kernel, grid, 128, 0, st, (const T*)y, place, weights, (const T*)add, (T*)out, copies, D);
+    launch_early(0, kernel, grid, 128, 0, st, (const T*)y, place, weights, (const T*)add, (T*)out, copies, D);
   });
   return launch_status("combine_experts");
 }

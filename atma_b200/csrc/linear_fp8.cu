@@ -179,6 +179,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
+  early_start();
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -682,7 +683,7 @@ int launch_pair(const CUtensorMap& x, const CUtensorMap& w, const Args& a, cudaS
   const int64_t tiles = (a.M / (2 * kBM) + (a.groups < a.M ? a.groups : a.M)) * n_tiles;       // at most
   ATMA_REQUIRE(tiles < INT32_MAX / 2, "linear_fp8: too many tiles");
   const int pairs = sm_count_of_current_device() / 2;
-  kern<<<2 * (unsigned)(tiles < pairs ? tiles : pairs), kPairThreads, kPairSmem, st>>>(x, w, a);
+  launch_early(0, kern, dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs)), dim3(kPairThreads), kPairSmem, st, x, w, a);
   return launch_status("linear_fp8 (many rows)");
 }
 

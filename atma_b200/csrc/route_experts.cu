@@ -538,6 +538,7 @@ route_experts_kernel(const __grid_constant__ RouteArgs a) {
 
 __global__ void __launch_bounds__(kRouteThreads)
 order_experts_kernel(const RouteArgs a) {
+  early_start();
   extern __shared__ uint8_t s_more[];
   // the chunks' counts, by as many threads an expert as there are, 16 loads of each under way
   const int tid = threadIdx.x, each = kRouteThreads / a.experts, e = tid % a.experts, part = tid / a.experts;
@@ -576,7 +577,7 @@ int launch_route(RouteArgs a, cudaStream_t st) {
   a.lanes = a.k < 32 && (a.groups == 1 || (size % V == 0 && (size / V & (size / V - 1)) == 0));
   auto kernel = a.experts == 32 * V ? route_experts_kernel<V, true> : route_experts_kernel<V, false>;
   const size_t more = a.chunks == 1 ? sizeof(OrderShared) : 0;
-  launch_early(a.tokens, kernel, a.chunks, kRouteThreads, more, st, a);
+  launch_early(0, kernel, a.chunks, kRouteThreads, more, st, a);
   return launch_status("route_experts");
 }
 
@@ -618,6 +619,6 @@ extern "C" int atma_route_experts(const float* logits, int64_t l_rs, const float
   else if (experts <= 256) rc = launch_route<8>(a, st);
   else rc = launch_route<16>(a, st);
   if (rc != ATMA_OK || chunks == 1) return rc;
-  order_experts_kernel<<<chunks, kRouteThreads, sizeof(OrderShared), st>>>(a);
+  launch_early(0, order_experts_kernel, dim3(chunks), dim3(kRouteThreads), sizeof(OrderShared), st, a);
   return launch_status("order_experts");
 }
