@@ -429,6 +429,23 @@ __device__ __forceinline__ float load_cluster(uint32_t addr) {
   return f;
 }
 
+// The largest of every token's values over the lanes, of token `lane` (modulo N, 16 or 32) in the end: N shuffles for N tokens.
+template <int N>
+__device__ __forceinline__ float token_max(float (&m)[N]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = N / 2; o > 0; o >>= 1) {
+    const bool upper = lane & o;
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const float keep = upper ? m[i + o] : m[i], send = upper ? m[i] : m[i + o];
+      m[i] = max_nan(keep, __shfl_xor_sync(0xffffffffu, send, o));
+    }
+  }
+  if (N == 16) m[0] = max_nan(m[0], __shfl_xor_sync(0xffffffffu, m[0], 16));
+  return m[0];
+}
+
 // ---- few rows --------------------------------------------------------------------------------------------
 constexpr int kRowsThreads = 192;
 
@@ -456,6 +473,7 @@ linear_fp8_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
   __shared__ int s_first[kMaxGroups + 1];
   __shared__ __align__(16) float s_scale[4][2][kHalves][NT];
   __shared__ float s_most[kGated ? 4 : 1][kGated ? NT : 1];
+  __shared__ __align__(8) float s_inverse[kGated ? 4 : 1][kGated ? NT : 2];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t rank, ranks;
@@ -564,27 +582,34 @@ linear_fp8_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
         if (!(ok = mbar_wait_warp(&acc_full[buf], (n / F::kBufs) & 1, abort))) break;
         tc_fence_after();
         const uint32_t at = tmem + (uint32_t(32 * quarter) << 16) + buf * kHalves * NT;
-        uint32_t r[kHalves][NT];
+        constexpr int kAtOnce = kHalves * NT <= 64 ? kHalves : 1;        // halves whose products a thread holds beside the sums
+        uint32_t r[kAtOnce][NT];
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h)
+        for (int h0 = 0; h0 < kHalves; h0 += kAtOnce) {
 #pragma unroll
-          for (int c = 0; c < NT; c += 16) tmem_ld16_nowait(at + h * NT + c, &r[h][c]);
-        tmem_ld_wait();
+          for (int h = 0; h < kAtOnce; ++h)
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h)
+            for (int c = 0; c < NT; c += 16) tmem_ld16_nowait(at + (h0 + h) * NT + c, &r[h][c]);
+          tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < NT; ++c) reg_fence(r[h][c]);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[buf]);
+          for (int h = 0; h < kAtOnce; ++h)
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h)
-#pragma unroll
-          for (int c = 0; c < NT; c += 4) {
-            const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(&sc[h][c]);
-            sum[h][c / 2] = fma2(pack2(__uint_as_float(r[h][c]), __uint_as_float(r[h][c + 1])), f.x, sum[h][c / 2]);
-            sum[h][c / 2 + 1] = fma2(pack2(__uint_as_float(r[h][c + 2]), __uint_as_float(r[h][c + 3])), f.y, sum[h][c / 2 + 1]);
+            for (int c = 0; c < NT; ++c) reg_fence(r[h][c]);
+          if (h0 + kAtOnce == kHalves) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[buf]);
           }
+#pragma unroll
+          for (int h = 0; h < kAtOnce; ++h)
+#pragma unroll
+            for (int c = 0; c < NT; c += 4) {
+              const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(&sc[h0 + h][c]);
+              uint64_t(&to)[NT / 2] = sum[h0 + h];
+              to[c / 2] = fma2(pack2(__uint_as_float(r[h][c]), __uint_as_float(r[h][c + 1])), f.x, to[c / 2]);
+              to[c / 2 + 1] = fma2(pack2(__uint_as_float(r[h][c + 2]), __uint_as_float(r[h][c + 3])), f.y, to[c / 2 + 1]);
+            }
+        }
       }
       if (!kGated || ranks > 1)
         if (!ok) break;
@@ -601,24 +626,42 @@ linear_fp8_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
         break;                              // a cluster has one tile
       }
       if constexpr (kGated) {
-        float v[NT];
+        constexpr int kPart = NT < 32 ? NT : 32;             // tokens whose largest values the lanes sort out among them
 #pragma unroll
-        for (int c = 0; c < NT; ++c) {
-          const float2 g = unpack2(sum[0][c / 2]), u = unpack2(sum[kHalves - 1][c / 2]);
-          v[c] = col < a.width ? gelu_tanh_16(c & 1 ? g.y : g.x) * (c & 1 ? u.y : u.x) : 0.f;
-          if (c < rows) {
-            const float most = warp_max_nan(fabsf(v[c]));
-            if (lane == 0) s_most[quarter][c] = most;
+        for (int i = 0; i < NT / 2; ++i) {
+          const float2 f = unpack2(gelu_gate_two(sum[0][i], sum[kHalves - 1][i]));
+          sum[0][i] = col < a.width ? pack2(f.x, f.y) : 0;   // what is behind the last column is another matrix's
+        }
+#pragma unroll
+        for (int t = 0; t < NT; t += kPart) {
+          float most[kPart];
+#pragma unroll
+          for (int c = 0; c < kPart; c += 2) {
+            const float2 f = unpack2(sum[0][(t + c) / 2]);
+            most[c] = fabsf(f.x);
+            most[c + 1] = fabsf(f.y);
           }
+          const float mine = token_max<kPart>(most);
+          if (lane < kPart) s_most[quarter][t + lane] = mine;
         }
         if (any_gave_up<128>(!ok || *abort)) break;
 #pragma unroll
-        for (int c = 0; c < NT; ++c)
-          if (c < rows) {
-            const float scale = fp8_scale(max_nan(max_nan(s_most[0][c], s_most[1][c]), max_nan(s_most[2][c], s_most[3][c])));
-            if (feature == 0) a.out_scales[(int64_t)(p.n0 / 128) * a.os_bs + p.m0 + c] = scale;
-            if (col < a.width) static_cast<uint8_t*>(a.out)[(int64_t)(p.m0 + c) * a.out_rs + col] = fp8_one_times(v[c], fp8_inverse(scale));
+        for (int t = lane; t < NT; t += 32) {
+          const float scale = fp8_scale(max_nan(max_nan(s_most[0][t], s_most[1][t]), max_nan(s_most[2][t], s_most[3][t])));
+          if (quarter == 0 && t < rows) a.out_scales[(int64_t)(p.n0 / 128) * a.os_bs + p.m0 + t] = scale;
+          s_inverse[quarter][t] = fp8_inverse(scale);
+        }
+        __syncwarp();
+        if (col < a.width) {
+          uint8_t* to = static_cast<uint8_t*>(a.out) + (int64_t)p.m0 * a.out_rs + col;
+#pragma unroll
+          for (int c = 0; c < NT; c += 2) {
+            const float2 inv = *reinterpret_cast<const float2*>(&s_inverse[quarter][c]), f = unpack2(sum[0][c / 2]);
+            const uint32_t q = fp8_two(f.x * inv.x, f.y * inv.y);
+            if (c < rows) to[c * a.out_rs] = (uint8_t)q;
+            if (c + 1 < rows) to[(c + 1) * a.out_rs] = (uint8_t)(q >> 8);
           }
+        }
         asm volatile("bar.sync 1, 128;" ::: "memory");       // s_most is read
       } else if (col < a.width) {
         T* out = static_cast<T*>(a.out) + (int64_t)p.m0 * a.out_rs + col;
