@@ -47,30 +47,33 @@ def route_experts(logits, top_k, *, score="softmax", bias=None, groups=1, top_gr
     looked at, those with the largest sum of their two best (None: all).  ``renormalize``: a token's weights are divided by their sum (zero where that is
     zero); ``scale`` multiplies them.  Equal ones: the lower index first.  NaN and -inf count as the least finite logit, inf as the
     largest; a choice is decided as in 64-bit arithmetic."""
-    here = _here(logits, bias)
-    if logits.ndim != 2 or not logits.is_floating_point():
+    here, shape = _here(logits, bias), logits.shape
+    if len(shape) != 2 or not logits.dtype.is_floating_point:
         raise ValueError("logits must be a (tokens, experts) matrix")
-    (tokens, experts), dev = logits.shape, logits.device
-    top_groups = groups if top_groups is None else top_groups
-    if score not in ("softmax", "sigmoid"):
+    (tokens, experts), dev = shape, logits.device
+    if top_groups is None:
+        top_groups = groups
+    if score != "softmax" and score != "sigmoid":
         raise ValueError(f"unknown score {score!r}; expected 'softmax' or 'sigmoid'")
     if not 0 < experts <= MAX_EXPERTS or not 0 < groups <= MAX_GROUPS or experts % groups or not 0 < top_groups <= groups:
         raise ValueError(f"{top_groups} of {groups} groups of {experts} experts (at most {MAX_EXPERTS} in {MAX_GROUPS} groups)")
     if not 0 < top_k <= min(MAX_TOP_K, experts // groups * top_groups):
         raise ValueError(f"{top_k} of {experts // groups * top_groups} experts (at most {MAX_TOP_K})")
-    if logits.dtype is not torch.float32 or logits.stride(1) != 1 and experts > 1 or logits.stride(0) < experts and tokens > 1:
-        logits = logits.float().contiguous()
+    step, unit = logits.stride()
+    if logits.dtype is not torch.float32 or unit != 1 and experts > 1 or step < experts and tokens > 1:
+        logits, step = logits.float().contiguous(), experts
     if bias is not None:
         if bias.shape != (experts,):
             raise ValueError(f"bias must have {experts} values, not the shape {tuple(bias.shape)}")
-        bias = bias.float().contiguous()
+        if bias.dtype is not torch.float32 or not bias.is_contiguous():
+            bias = bias.float().contiguous()
     lib, n, i32 = _lib.load_decoder(), tokens * top_k, torch.int32
     ids = _new((tokens, top_k), (top_k, 1), device=dev, dtype=i32)
     weights = _new((tokens, top_k), (top_k, 1), device=dev, dtype=torch.float32)
     plan = _new((2 * n + experts + 1,), (1,), device=dev, dtype=i32)
     ints, at = lib.atma_route_scratch_ints(tokens, experts), plan.data_ptr()
     scratch = _new((ints,), (1,), device=dev, dtype=i32) if ints else None
-    rc = lib.atma_route_experts(logits.data_ptr(), logits.stride(0) if tokens > 1 else experts, None if bias is None else bias.data_ptr(), ids.data_ptr(),
+    rc = lib.atma_route_experts(logits.data_ptr(), step if tokens > 1 else experts, None if bias is None else bias.data_ptr(), ids.data_ptr(),
                                 weights.data_ptr(), at, at + 4 * n, at + 8 * n, None if scratch is None else scratch.data_ptr(), tokens, experts, top_k,
                                 score == "sigmoid", groups, top_groups, bool(renormalize), scale, _stream(here))
     if rc:
