@@ -118,7 +118,8 @@ __device__ __forceinline__ bool keep_groups(typename Ordered<F>::type (&key)[V],
     const U most = warp_most(best);
     const uint32_t holders = __ballot_sync(0xffffffffu, best == most);
     const U next = warp_most(lane == __ffs(holders) - 1 ? second : best);
-    const F sum = next == 0 ? value_of(most) : value_of(most) + value_of(next);      // a group of one expert has no second
+    // a group of one expert has no second; inf and -inf are inf
+    const F sum = next == 0 || value_of(most) == F(INFINITY) ? value_of(most) : value_of(most) + value_of(next);
     if (lane == (g & 31)) mine[g >> 5] = ordered(sum);
   }
   uint64_t left = 0;
@@ -141,7 +142,7 @@ __device__ __forceinline__ bool keep_groups(typename Ordered<F>::type (&key)[V],
   }
 #pragma unroll
   for (int v = 0; v < V; ++v)
-    if (e0 + v < a.experts && !(left >> ((e0 + v) / size) & 1)) key[v] = ordered(-F(INFINITY));
+    if (e0 + v < a.experts && !(left >> ((e0 + v) / size) & 1)) key[v] = 0;        // below -inf, which a bias may give experts that stay
   return settled;
 }
 
@@ -185,7 +186,7 @@ __device__ __noinline__ Chosen choose(const float* row, int e0, const RouteArgs&
     for (int v = 0; v < V; ++v)
       if (key[v] > best) { best = key[v]; at = s[v]; where = v; }
     const U most = warp_most(best);
-    if (check && n > 0) {
+    if (check && n > 0 && most != 0) {                       // 0: none is left
       const float p = (float)value_of(last), q = (float)value_of(most);
       settled = settled && p - q > kKeyError * (fabsf(p) + 1.f);       // also where both are -inf
     }
@@ -278,7 +279,7 @@ __device__ __noinline__ bool group_goes_in_64(const float* row, int e0, float m,
     second = fmax(fmax(second, c), fmin(best, b));
     best = fmax(best, b);
   }
-  const double both = V * lanes == 1 ? best : best + second;
+  const double both = V * lanes == 1 || best == INFINITY ? best : best + second;      // inf and -inf are inf
   int above = 0;
 #pragma unroll 1
   for (int from = 0; from < a.groups * lanes; from += lanes) {
@@ -359,8 +360,8 @@ __device__ __forceinline__ bool choose_fast(const float (&z)[V], const float (&b
   uint32_t word[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    word[v] = (ordered(out ? -FLT_MAX : key[v]) & ~kPlace) | (kPlace - (uint32_t)(e0 + v));
-    if (!kFull && v >= own) word[v] = 0;    // nobody's: below all others
+    word[v] = (ordered(key[v]) & ~kPlace) | (kPlace - (uint32_t)(e0 + v));
+    if (out || (!kFull && v >= own)) word[v] = 0;            // not to be had: below all others
   }
   sort_words<V>(word);
   auto take = [&]() {                       // the largest word that is left

@@ -75,10 +75,13 @@ def route(logits, top_k, score="softmax", bias=None, groups=1, top_groups=1, ren
         key = list(z) if bias is None and groups == 1 else [s[i] + (0.0 if bias is None else float(bias[i])) for i in range(n)]
         if groups > 1:
             size = n // groups
-            of = [sum(sorted(key[g * size:(g + 1) * size], reverse=True)[:2]) for g in range(groups)]
+            two = [sorted(key[g * size:(g + 1) * size], reverse=True)[:2] for g in range(groups)]
+            of = [t[0] if t[0] == math.inf else sum(t) for t in two]
             kept = sorted(range(groups), key=lambda g: (-of[g], g))[:top_groups]
-            key = [k if i // size in kept else -math.inf for i, k in enumerate(key)]
-        best = sorted(range(n), key=lambda i: (-key[i], i))[:top_k]
+            left = [i for i in range(n) if i // size in kept]                        # also where a bias leaves their keys at -inf
+        else:
+            left = range(n)
+        best = sorted(left, key=lambda i: (-key[i], i))[:top_k]
         w = [s[i] for i in best]
         if renormalize:
             w = [v / sum(w) if sum(w) > 0 else 0.0 for v in w]

@@ -114,6 +114,27 @@ def test_route_experts_with_groups_that_a_bias_rules_out_or_forces(score, groups
     check_order(r)
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts, groups, top_groups, k", [(16, 4, 1, 4), (32, 4, 2, 12), (64, 8, 2, 16), (12, 4, 2, 6), (200, 10, 2, 40), (128, 64, 3, 5)])
+def test_route_experts_stays_in_the_best_groups_where_a_bias_rules_out_their_experts(score, experts, groups, top_groups, k):
+    """A kept group with one finite key, the rest at -inf: those, and none of the groups that go, fill up the choice."""
+    size = experts // groups
+    x, bias = rand((20, experts), 8), torch.zeros(experts)
+    for g in range(groups - top_groups, groups):
+        bias[g * size:(g + 1) * size] = -math.inf
+        bias[g * size] = bias[g * size + 1] = 5.0
+    for b in (bias, torch.where(bias == 5.0, torch.tensor(math.inf), bias)):
+        r = routing().route_experts(x.cuda(), k, score=score, bias=b.cuda(), groups=groups, top_groups=top_groups)
+        assert all(e // size >= groups - top_groups for row in r.ids.tolist() for e in row)
+        assert r.ids.tolist() == O.route(x, k, score, b, groups, top_groups)[0]
+        check_order(r)
+    b = bias.clone()                                         # an infinity beside -inf makes its group the best
+    b[:size] = -math.inf
+    b[0] = math.inf
+    r = routing().route_experts(x.cuda(), k, score=score, bias=b.cuda(), groups=groups, top_groups=top_groups)
+    assert r.ids.tolist() == O.route(x, k, score, b, groups, top_groups)[0]
+
+
 def test_route_experts_takes_strided_and_16_bit_logits():
     x = rand((50, 40), 2)
     r = routing().route_experts(x.cuda()[:, 4:36], 3)
