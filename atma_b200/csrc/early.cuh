@@ -8,8 +8,12 @@
 // it is a request to bring memory into L2, which is coherent and so may be early for whatever is written there later.
 // Inputs are not declared __restrict__: read-only loads could be moved in front of the wait.
 //
-// Only steps of a few rows are launched so: their products are this library's too.  Between a library's kernels, which neither
-// release early nor start early, it gives nothing (64 rows of Zemivik: 573 us a step without, 576 with).
+// Steps of a few rows are launched so, whose products are this library's too.  Between a library's kernels, which neither
+// release early nor start early, it gives nothing (64 rows of Zemivik: 573 us a step without, 576 with).  The operators in 8 bits and of
+// experts, whose products are this library's at any size, pass 0 for the step's rows: always.
+//
+// One thread's release counts for its CTA.  So a kernel that takes TMEM in front of the wait shares its SM, by what it asks of shared memory
+// and of TMEM, with no more CTAs of such kernels than there are columns for: none then waits for columns of one that waits for it.
 #pragma once
 
 #include <cuda_runtime.h>

@@ -93,9 +93,11 @@ def expert_mlp(x, w_gate_up, w_down, routes, add=None, dtype=torch.bfloat16):
     if w_gate_up.values.shape != (experts, 2, ff, width) or w_down.values.shape != (experts, width, ff) or chosen != tokens:
         raise ValueError(f"weights of the shapes {tuple(w_gate_up.shape)} and {tuple(w_down.shape)} do not fit rows {tuple(x.shape)} and "
                          f"{tuple(routes.ids.shape)} choices of {experts} experts")
+    if routes.weights.shape != routes.ids.shape or routes.weights.dtype is not torch.float32 or not routes.weights.is_contiguous():
+        raise ValueError("the routes' weights must be (tokens, top_k) float32, contiguous")
     if dtype not in _TYPES or add is not None and (add.shape != (tokens, width) or add.dtype is not dtype or not add.is_contiguous()):
         raise ValueError("bfloat16 or float32, add contiguous in the same type")
-    here, dev = _here(x.values, w_gate_up.values, w_down.values, routes.ids, add), x.values.device
+    here, dev = _here(x.values, w_gate_up.values, w_down.values, routes._plan, routes.weights, add), x.values.device
     lib, code = _lib.load_decoder(), _lib.DTYPE_CODE[dtype]
     out = _new((tokens, width), (width, 1), device=dev, dtype=dtype)
     scratch = _new((lib.atma_expert_mlp_scratch_bytes(tokens, top_k, width, ff, code),), (1,), device=dev, dtype=torch.uint8)

@@ -131,6 +131,17 @@ def test_refused_arguments(anywhere):
             pytest.fail(f"call {i} was not refused")
 
 
+def test_routes_with_other_weights(anywhere):
+    """A user may put weights of their own into the routes; what the kernels could not read is refused."""
+    f, e = anywhere
+    r, stack = f.Fp8Rows(torch.zeros(4, 256, dtype=f.E4M3), torch.zeros(4, 2)), (f.Fp8Weight.of(torch.zeros(6, 2, 32, 256)), f.Fp8Weight.of(torch.zeros(6, 256, 32)))
+    w = torch.zeros(4, 2)
+    for bad in (w.double(), w.bfloat16(), w[:, :1], w.t().contiguous().t(), w[:3], w[0]):
+        routes = e.Routes(torch.zeros(4, 2, dtype=torch.int32), bad, 6, torch.zeros(23, dtype=torch.int32))
+        with pytest.raises(ValueError, match="weights"):
+            e.expert_mlp(r, *stack, routes)
+
+
 @pytest.fixture(scope="module")
 def lib():
     from atma_b200 import _lib

@@ -222,6 +222,55 @@ def test_expert_mlp_a_broken_token_stays_by_itself_and_the_order_of_tokens_does_
     assert run(h[:0], logits[:0]).shape == (0, 256)
 
 
+def test_expert_mlp_of_no_tokens_and_with_other_weights():
+    e, f = routing(), ops()
+    w_in, w_out = f.Fp8Weight.of(rand((4, 2, 64, 96), 1).cuda()), f.Fp8Weight.of(rand((4, 96, 64), 2).cuda())
+    x = f.quantize_rows(rand((6, 96), 3).cuda())
+    assert e.expert_mlp(x[:0], w_in, w_out, e.route_experts(torch.empty(0, 4, device="cuda"), 2)).shape == (0, 96)
+    r = e.route_experts(rand((6, 4), 4).cuda(), 2)
+    whole = e.expert_mlp(x, w_in, w_out, r, dtype=torch.float32)
+    r.weights = 2 * r.weights                                # exact: so is the doubled sum
+    assert torch.equal(e.expert_mlp(x, w_in, w_out, r, dtype=torch.float32), 2 * whole)
+
+
+def test_operators_behind_copies_and_joined_streams_in_a_graph():
+    """What stands in front of a launch that may begin early is a memset, a copy or another stream's kernel."""
+    from atma_b200.decoder_ops import linear
+    f = ops()
+    src, w = rand((40, 256), 1).cuda(), f.Fp8Weight.of(rand((128, 256), 2).cuda())
+    a, b = torch.empty_like(src), torch.empty_like(src)
+    out = torch.empty(40, 128, device="cuda")
+
+    def run(side):
+        here = torch.cuda.current_stream()
+        a.zero_()
+        qa = f.quantize_rows(a)
+        b.copy_(src)
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            b.mul_(0.5)
+            qb = f.quantize_rows(b)
+        a.copy_(src)
+        here.wait_stream(side)
+        f.linear_fp8(qb, w, out=out)
+        return out + f.linear_fp8(qa, w, dtype=torch.float32) + linear(f.quantize_rows(a), w).float()
+
+    side = torch.cuda.Stream()
+    run(side)
+    torch.cuda.synchronize()
+    expected = run(side).clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        result = run(side)
+    for i in range(3):
+        src.mul_(2.0)                                        # scales double, values stay
+        result.fill_(math.nan)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(result, expected * 2.0 ** (i + 1))
+
+
 def test_norm_routing_and_experts_in_a_graph():
     """The layer's run of operators, captured: replays on other inputs do what the calls do."""
     e, f = routing(), ops()
