@@ -103,15 +103,19 @@ __device__ __forceinline__ Place place_of(int tile, const int* s_first, const Ar
 }
 
 // gelu_tanh(gate) * up of two values each: gate up / (1 + e^-2u), u = sqrt(2 / pi) (z + 0.044715 z^3), by the fast exponential and one
-// reciprocal for both.  The exponent stops at 2^63, where the product of two denominators still fits: results below that are
+// reciprocal for both if they are of one row (kOne): a value's last bits then depend on the other one, which is nothing that a row may
+// see of its neighbour.  The exponent stops at 2^63, where the product of two denominators still fits: results below that are
 // off by 1e-19 of gate * up.  Else off by what gelu_tanh_16 is, 6e-6 at most.
+template <bool kOne>
 __device__ __forceinline__ uint64_t gelu_gate_two(uint64_t gate, uint64_t up) {
   constexpr float kLinear = -2.30220819814f, kCubic = kLinear * 0.044715f;         // -2 sqrt(2 / pi) log2(e)
   const float2 x = unpack2(mul2(fma2(mul2(gate, gate), pack2(kCubic, kCubic), pack2(kLinear, kLinear)), gate));
   float e0, e1;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(fminf(x.x, 63.f)));
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(fminf(x.y, 63.f)));
-  const float a = 1.f + e0, b = 1.f + e1, r = __fdividef(1.f, a * b);
+  const float a = 1.f + e0, b = 1.f + e1;
+  if constexpr (!kOne) return mul2(mul2(gate, up), pack2(__fdividef(1.f, a), __fdividef(1.f, b)));
+  const float r = __fdividef(1.f, a * b);
   return mul2(mul2(gate, up), pack2(r * b, r * a));
 }
 
@@ -323,7 +327,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
         const int f0 = p.n0 + 64 * side;
         float most = 0.f;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) sum[i] = gelu_gate_two(sum[i], sum[32 + i]);
+        for (int i = 0; i < 32; ++i) sum[i] = gelu_gate_two<true>(sum[i], sum[32 + i]);
         if (p.n0 + 128 > a.width)           // what is behind the last column is another matrix's
 #pragma unroll
           for (int i = 0; i < 64; i += 2) {
@@ -629,7 +633,7 @@ linear_fp8_rows_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
         constexpr int kPart = NT < 32 ? NT : 32;             // tokens whose largest values the lanes sort out among them
 #pragma unroll
         for (int i = 0; i < NT / 2; ++i) {
-          const float2 f = unpack2(gelu_gate_two(sum[0][i], sum[kHalves - 1][i]));
+          const float2 f = unpack2(gelu_gate_two<false>(sum[0][i], sum[kHalves - 1][i]));
           sum[0][i] = col < a.width ? pack2(f.x, f.y) : 0;   // what is behind the last column is another matrix's
         }
 #pragma unroll

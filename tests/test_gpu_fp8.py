@@ -264,6 +264,18 @@ def test_gelu_gated_linear_fp8(M, N, K):
     assert (near | (mine == q)).all()
 
 
+@pytest.mark.parametrize("M, K", [(9, 512), (30, 300), (60, 512), (60, 2048), (120, 512), (300, 512)])
+def test_a_row_does_not_depend_on_its_neighbours(M, K):
+    """Rows in another order: each has the same bits."""
+    f = ops()
+    x, w, g = rand((M, K), M).cuda(), f.Fp8Weight.of(rand((200, K), 1, K ** -0.5).cuda()), f.Fp8Weight.of(rand((2, 1000, K), 2, 2 * K ** -0.5).cuda())
+    p = torch.randperm(M, generator=torch.Generator().manual_seed(3)).cuda()
+    a, b = f.quantize_rows(x), f.quantize_rows(x[p])
+    assert torch.equal(f.linear_fp8(a, w, dtype=torch.float32)[p], f.linear_fp8(b, w, dtype=torch.float32))
+    a, b = f.gelu_gated_linear_fp8(a, g), f.gelu_gated_linear_fp8(b, g)
+    assert torch.equal(a.scales[p], b.scales) and torch.equal(a.values.view(torch.uint8)[p], b.values.view(torch.uint8))
+
+
 def test_products_leave_no_status():
     """The bounded waits of the tensor-core kernels: none of this file's launches ran one out."""
     from atma_b200 import decoder_ops
