@@ -23,7 +23,7 @@
 // that a stage is all weight.  Bound by reading that: two CTAs an SM with 100 KB of copies in flight each.  128 rows of 64 experts, 2048 x
 // 2048 gated 43 us, 6.2 TB/s; 2048 x 1024 25 us, 5.4.  Where a dense product has too few tiles for that, a cluster shares one: every CTA takes
 // its part of the columns, and each then adds up what all of them have for some of the tokens, from their shared memory and in their
-// order.  8192 x 2048: 4 rows 9.8 us, 64 rows 13.9 (20 with a token's words read one after another), 128 rows 16.4; 200 rows take the other kernel, 16.5.
+// order.  8192 x 2048: 4 rows 9.8 us, 64 rows 11.9 (20 with a token's words read one after another), 128 rows by the other kernel 12.6.
 //
 // Every mbarrier wait is bounded; on expiry the CTAs free their TMEM, return and leave a status word for the host.
 #include "common.cuh"
@@ -757,10 +757,26 @@ int launch_rows(const CUtensorMap& x, const CUtensorMap& w, const Args& a, cudaS
   return launch_status("linear_fp8 (few rows)");
 }
 
+// Which kernel, by a group's rows if all have as many.  The pair kernel reads a weight once for 256 rows, but a pair walks all of K by itself:
+// `chain` blocks one behind another, 5.6 us and 0.4 a block where the weights are in time.  Few rows are bound by the weights, or share K.
+// Either one, us, few rows / many rows:
+//   one weight 8192 x 2048 (chain 16)   64 rows 11.9 / 12.4   80 rows 13.6 / 12.4;   4096 x 4096 (32)   80 rows 13.1 / 18.2
+//   gated, 2 x 4096 x 2048 (16)         24 rows 13.8 / 14.2   40 rows 15.2 / 13.0;   2 x 1024 x 8192 (64)   80 rows 25.7 / 30.6
+//   64 experts of 2 x 1024 x 2048, the whole feed-forward   32 rows each 105 / 117   48 119 / 119   64 141 / 129   125 203 / 156;
+//   its second product   48 119 / 130   64 141 / 144   96 174 / 165
+template <bool kGated>
+bool many_rows(const Args& a, int each) {
+  const int pairs = sm_count_of_current_device() / 2, wide = kGated ? 128 : 256;
+  const int64_t tiles = (int64_t)a.groups * ((each + 255) / 256) * ((a.width + wide - 1) / wide), turns = (tiles + pairs - 1) / pairs, chain = turns * a.kb;
+  if (each > 128) return true;
+  const bool spread = a.starts != nullptr || turns > 1;      // weights come over all SMs either way
+  if (kGated) return (each > 48 && spread) || (each >= 32 && chain <= 32);
+  return each > 64 && (spread || chain <= 20);
+}
+
 template <typename T, bool kGated>
 int launch(const atma_fp8_args& f, const Args& a, cudaStream_t st) {
-  // rows of a group, if all have as many; measured above: 128 rows by 64 16.4 us, 200 by the pair kernel 16.5
-  const int each = (a.M + a.groups - 1) / a.groups, nt = each <= 16 ? 16 : each <= 32 ? 32 : each <= 128 ? 64 : 0;
+  const int each = (a.M + a.groups - 1) / a.groups, nt = many_rows<kGated>(a, each) ? 0 : each <= 16 ? 16 : each <= 32 ? 32 : 64;
   CUtensorMap x, w;
   int rc = make_tmap_8bit_rows(&x, f.x, a.M, f.x_rs, a.K, nt > 0 ? nt : kBM);
   if (rc == ATMA_OK) rc = make_tmap_8bit_rows(&w, f.w, (uint64_t)a.groups * f.N, f.w_rs, a.K, nt > 0 ? kBM : kBM / 2);

@@ -184,6 +184,12 @@ def test_expert_mlp(tokens, n, k, width, ff, dtype):
         assert y.dtype == dtype and ((y.cpu().double() - want).abs() <= off + 1e-40).all()
 
 
+@pytest.mark.parametrize("tokens, n, k, width, ff", [(90, 5, 2, 264, 136), (100, 4, 2, 256, 300), (140, 4, 2, 136, 128), (33, 2, 2, 1032, 96)])
+def test_expert_mlp_on_both_sides_of_the_choice_of_kernels(tokens, n, k, width, ff):
+    """36, 50, 70 and 33 rows an expert."""
+    test_expert_mlp(tokens, n, k, width, ff, torch.bfloat16)
+
+
 def test_expert_mlp_where_all_tokens_go_to_one_expert_and_others_have_none():
     e, f = routing(), ops()
     logits = torch.zeros(260, 9)

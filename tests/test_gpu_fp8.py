@@ -276,6 +276,12 @@ def test_a_row_does_not_depend_on_its_neighbours(M, K):
     assert torch.equal(a.scales[p], b.scales) and torch.equal(a.values.view(torch.uint8)[p], b.values.view(torch.uint8))
 
 
+@pytest.mark.parametrize("M, N, K", [(31, 300, 700), (32, 300, 700), (33, 130, 4224), (65, 520, 2560), (65, 520, 2688), (100, 19000, 200), (50, 9500, 136)])
+def test_products_on_both_sides_of_the_choice_of_kernels(M, N, K):
+    test_linear_fp8(M, N, K, torch.float32)
+    test_gelu_gated_linear_fp8(M, N // 2, K)
+
+
 def test_products_leave_no_status():
     """The bounded waits of the tensor-core kernels: none of this file's launches ran one out."""
     from atma_b200 import decoder_ops
