@@ -1,5 +1,6 @@
 // The experts' feed-forwards in one call: rows to the places of their experts, both products, the weighted sum.
 #include "common.cuh"
+#include "linear_fp8.cuh"
 #include "../../include/atma_decoder.h"
 
 namespace atma {
@@ -9,6 +10,12 @@ namespace {
 int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 struct Parts { int64_t rows, row_scales, act, act_scales, y, all; };             // offsets in the scratch memory, bytes
+
+// Experts' results before they are summed: fp32 where that is little (1 us of 124 with 512 tokens, 8 of 64 experts, 2048 / 1024), else in the
+// activation type.  A bf16 sum's error has a 2-norm of 2.3e-3 with that rounding and of 1.7e-3 without; fp32 takes 142 us instead of 130 with
+// 1000 tokens, 695 instead of 602 with 8192.
+constexpr int64_t kWideBytes = 32 << 20;
+bool wide_results(int64_t rows, int width, int dtype) { return dtype == ATMA_F32 || rows * width * 4 <= kWideBytes; }
 
 // Values of 128 bytes more than a row's are never needed: rows start on 16-byte boundaries, parts on 256-byte ones.
 Parts parts_of(int64_t rows, int width, int ff, int size) {
@@ -29,7 +36,7 @@ using namespace atma;
 
 extern "C" int64_t atma_expert_mlp_scratch_bytes(int tokens, int copies, int width, int ff, int dtype) {
   if (tokens <= 0 || copies <= 0 || width <= 0 || ff <= 0) return 0;
-  return parts_of((int64_t)tokens * copies, width, ff, dtype == ATMA_F32 ? 4 : 2).all;
+  return parts_of((int64_t)tokens * copies, width, ff, wide_results((int64_t)tokens * copies, width, dtype) ? 4 : 2).all;
 }
 
 extern "C" int atma_expert_mlp(const atma_expert_args* args, void* scratch, void* stream) {
@@ -42,7 +49,8 @@ extern "C" int atma_expert_mlp(const atma_expert_args* args, void* scratch, void
   ATMA_REQUIRE(scratch != nullptr && (reinterpret_cast<uintptr_t>(scratch) & 255) == 0, "expert_mlp: scratch memory must be 256-byte aligned");
   ATMA_REQUIRE(a.place != nullptr && a.starts != nullptr && a.weights != nullptr && a.out != nullptr, "expert_mlp: null tensors");
   const int rows = a.tokens * a.copies;
-  const Parts p = parts_of(rows, a.width, a.ff, a.dtype == ATMA_F32 ? 4 : 2);
+  const bool wide = wide_results(rows, a.width, a.dtype);
+  const Parts p = parts_of(rows, a.width, a.ff, wide ? 4 : 2);
   uint8_t* s = static_cast<uint8_t*>(scratch);
   const int64_t x_rs = round_up(a.width, 16), act_rs = round_up(a.ff, 16);
   float *row_scales = reinterpret_cast<float*>(s + p.row_scales), *act_scales = reinterpret_cast<float*>(s + p.act_scales);
@@ -53,8 +61,8 @@ extern "C" int atma_expert_mlp(const atma_expert_args* args, void* scratch, void
   rc = atma_linear_fp8(&up, stream);
   if (rc != ATMA_OK) return rc;
   const atma_fp8_args down = {s + p.act, act_rs, act_scales, rows, a.w_down, a.w_down_rs, a.w_down_scales, s + p.y, a.width, nullptr, 0,
-                              a.starts, rows, a.width, a.ff, a.experts, 0, a.dtype};
+                              a.starts, rows, a.width, a.ff, a.experts, 0, wide ? ATMA_F32 : ATMA_BF16};
   rc = atma_linear_fp8(&down, stream);
   if (rc != ATMA_OK) return rc;
-  return atma_combine_experts(s + p.y, a.place, a.weights, a.add, a.out, a.tokens, a.copies, a.width, a.dtype, stream);
+  return combine_experts(s + p.y, wide, a.place, a.weights, a.add, a.out, a.tokens, a.copies, a.width, a.dtype, (cudaStream_t)stream);
 }

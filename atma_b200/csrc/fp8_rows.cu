@@ -10,6 +10,7 @@
 #include "common.cuh"
 #include "early.cuh"
 #include "fp8.cuh"
+#include "linear_fp8.cuh"
 #include "../../include/atma_decoder.h"
 
 namespace atma {
@@ -270,9 +271,9 @@ scatter_rows_fp8_kernel(const uint8_t* q, int64_t q_rs, const float* scales, int
 
 // ---- the weighted sum of a token's results -------------------------------------------------------------------
 // Eight results of a token at a time, all of them asked for before the first is summed: a row is 4 KB, and a token by itself is all latency.
-template <typename T, int VEC>
+template <typename Y, typename T, int VEC>
 __global__ void __launch_bounds__(128)
-combine_experts_kernel(const T* y, const int32_t* place, const float* weights, const T* add, T* out, int copies, int D) {
+combine_experts_kernel(const Y* y, const int32_t* place, const float* weights, const T* add, T* out, int copies, int D) {
   early_start();
   constexpr int kAtOnce = 8;
   const int64_t row = blockIdx.x;
@@ -287,11 +288,11 @@ combine_experts_kernel(const T* y, const int32_t* place, const float* weights, c
     const bool mine = lane < kAtOnce && j0 + lane < copies;
     const int at = mine ? place[row * copies + j0 + lane] : 0;
     const float weight = mine ? weights[row * copies + j0 + lane] : 0.f;
-    Some<T, VEC> p[kAtOnce];
+    Some<Y, VEC> p[kAtOnce];
 #pragma unroll
     for (int j = 0; j < kAtOnce; ++j) {
       const int64_t from = __shfl_sync(0xffffffffu, at, j);
-      if (j0 + j < copies && c < D) p[j] = *reinterpret_cast<const Some<T, VEC>*>(y + from * D + c);
+      if (j0 + j < copies && c < D) p[j] = *reinterpret_cast<const Some<Y, VEC>*>(y + from * D + c);
     }
 #pragma unroll
     for (int j = 0; j < kAtOnce; ++j) {
@@ -308,9 +309,31 @@ combine_experts_kernel(const T* y, const int32_t* place, const float* weights, c
   *reinterpret_cast<Some<T, VEC>*>(out + row * D + c) = p;
 }
 
+template <typename Y, typename T>
+void launch_combine(const void* y, const int32_t* place, const float* weights, const void* add, void* out, int rows, int copies, int D, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(Y);                          // 16 bytes of y a thread
+  const bool vec = D % V == 0 && fits(y, 16) && fits(add, V * sizeof(T)) && fits(out, V * sizeof(T));
+  const dim3 grid((unsigned)rows, (unsigned)((D + 128 * (vec ? V : 1) - 1) / (128 * (vec ? V : 1))));
+  auto* kernel = vec ? combine_experts_kernel<Y, T, V> : combine_experts_kernel<Y, T, 1>;
+  launch_early(0, kernel, grid, 128, 0, st, (const Y*)y, place, weights, (const T*)add, (T*)out, copies, D);
+}
+
 bool rows_ok(int64_t rows, int64_t width) { return rows >= 0 && rows <= INT32_MAX / 2 && width > 0 && width <= (1 << 24); }
 
 }  // namespace
+
+// See linear_fp8.cuh.
+int combine_experts(const void* y, bool wide, const int32_t* place, const float* weights, const void* add, void* out, int rows, int copies, int D,
+                    int dtype, cudaStream_t st) {
+  ATMA_REQUIRE(dtype == ATMA_F32 || dtype == ATMA_BF16, "combine_experts: unsupported dtype %d", dtype);
+  ATMA_REQUIRE(rows_ok(rows, D) && D <= 128 * 65535 && copies > 0 && copies <= 1024 && (int64_t)rows * copies <= INT32_MAX, "combine_experts: bad shape");
+  if (rows == 0) return ATMA_OK;
+  ATMA_REQUIRE(y != nullptr && place != nullptr && weights != nullptr && out != nullptr, "combine_experts: null tensors");
+  if (dtype == ATMA_F32) launch_combine<float, float>(y, place, weights, add, out, rows, copies, D, st);
+  else if (wide) launch_combine<float, __nv_bfloat16>(y, place, weights, add, out, rows, copies, D, st);
+  else launch_combine<__nv_bfloat16, __nv_bfloat16>(y, place, weights, add, out, rows, copies, D, st);
+  return launch_status("combine_experts");
+}
 }  // namespace atma
 
 using namespace atma;
@@ -381,18 +404,5 @@ extern "C" int atma_scatter_rows_fp8(const void* q, int64_t q_rs, const float* s
 
 extern "C" int atma_combine_experts(const void* y, const int32_t* place, const float* weights, const void* add, void* out, int rows,
                                     int copies, int D, int dtype, void* stream) {
-  ATMA_REQUIRE(dtype == ATMA_F32 || dtype == ATMA_BF16, "combine_experts: unsupported dtype %d", dtype);
-  ATMA_REQUIRE(rows_ok(rows, D) && copies > 0 && copies <= 1024 && (int64_t)rows * copies <= INT32_MAX, "combine_experts: bad shape");
-  if (rows == 0) return ATMA_OK;
-  ATMA_REQUIRE(y != nullptr && place != nullptr && weights != nullptr && out != nullptr, "combine_experts: null tensors");
-  cudaStream_t st = (cudaStream_t)stream;
-  ATMA_FP8_DISPATCH(dtype, T, {
-    constexpr int V = 16 / sizeof(T);
-    const bool vec = D % V == 0 && fits(y, 16) && fits(add, 16) && fits(out, 16);
-    const dim3 grid((unsigned)rows, (unsigned)((D + 128 * (vec ? V : 1) - 1) / (128 * (vec ? V : 1))));
-    ATMA_REQUIRE(grid.y <= 65535, "combine_experts: rows of %d channels", D);
-    auto* kernel = vec ? combine_experts_kernel<T, V> : combine_experts_kernel<T, 1>;
-    launch_early(0, kernel, grid, 128, 0, st, (const T*)y, place, weights, (const T*)add, (T*)out, copies, D);
-  });
-  return launch_status("combine_experts");
+  return combine_experts(y, false, place, weights, add, out, rows, copies, D, dtype, (cudaStream_t)stream);
 }

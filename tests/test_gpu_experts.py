@@ -190,6 +190,28 @@ def test_expert_mlp_on_both_sides_of_the_choice_of_kernels(tokens, n, k, width, 
     test_expert_mlp(tokens, n, k, width, ff, torch.bfloat16)
 
 
+@pytest.mark.parametrize("tokens", [1, 30, 300])
+def test_expert_mlp_rounds_small_sums_once(tokens):
+    """What is summed is fp32 for either result: the 16-bit one is the other, rounded."""
+    e, f = routing(), ops()
+    w_in, w_out = weight8((8, 2, 128, 256), 1)[0], weight8((8, 256, 128), 2)[0]
+    x = f.quantize_rows(rand((tokens, 256), 1, dtype=torch.bfloat16).cuda())
+    routes = e.route_experts(rand((tokens, 8), 3).cuda(), 8)
+    fine = e.expert_mlp(x, w_in, w_out, routes, dtype=torch.float32)
+    assert torch.equal(e.expert_mlp(x, w_in, w_out, routes), fine.bfloat16())
+
+
+def test_expert_mlp_of_more_results_than_are_kept_in_32_bits():
+    """34 MB of them in fp32.  With one expert a token, whose weight is 1, rounding twice is rounding once."""
+    e, f = routing(), ops()
+    w_in, w_out = weight8((8, 2, 128, 256), 1)[0], weight8((8, 256, 128), 2)[0]
+    x = f.quantize_rows(rand((33000, 256), 1, dtype=torch.bfloat16).cuda())
+    routes = e.route_experts(rand((33000, 8), 3).cuda(), 1)
+    assert (routes.weights == 1).all()
+    fine = e.expert_mlp(x, w_in, w_out, routes, dtype=torch.float32)
+    assert torch.equal(e.expert_mlp(x, w_in, w_out, routes), fine.bfloat16())
+
+
 def test_expert_mlp_where_all_tokens_go_to_one_expert_and_others_have_none():
     e, f = routing(), ops()
     logits = torch.zeros(260, 9)
