@@ -734,6 +734,41 @@ int launch_pair(const CUtensorMap& x, const CUtensorMap& w, const Args& a, cudaS
   return launch_status("linear_fp8 (many rows)");
 }
 
+// Clusters of `ranks` CTAs that run at once.  With a CTA an SM fewer of them find a place than of its CTAs, since a cluster's lie in one GPC, and a
+// second turn of clusters costs more than what sharing K gives (gated 1024 x 8192, 256 rows: 31.6 us by eight, 23.3 by four); that is asked
+// for once per device.  With two CTAs an SM it is not so: what the query gives is 24 us with 192 rows of 2048 x 8192, CTAs alone 17.5.
+template <int NT, bool kGated>
+int64_t clusters_at_once(int ranks) {
+  using F = Few<NT, kGated>;
+  static int cached[64][4] = {};
+  const int64_t guess = F::kCtas * (int64_t)sm_count_of_current_device() / ranks;
+  int dev = 0, at = ranks == 2 ? 1 : ranks == 4 ? 2 : 3, n = 0;
+  if (F::kCtas > 1 || ranks == 1 || cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return guess;
+  if (cached[dev][at] == 0) {
+    auto kern = linear_fp8_rows_kernel<float, NT, kGated>;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = ranks; attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(ranks); c.blockDim = dim3(kRowsThreads); c.dynamicSmemBytes = F::kSmem; c.attrs = &attr; c.numAttrs = 1;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kern, &c) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      return guess;
+    }
+    cached[dev][at] = n;                    // the same value from every host thread
+  }
+  return cached[dev][at];
+}
+
+// CTAs that share a tile's columns: as many as find a place with all tiles, four blocks each at least.
+template <int NT, bool kGated>
+int ranks_of(int64_t tiles, int kb) {
+  int ranks = 1;
+  while (ranks < 8 && 4 * 2 * ranks <= kb && tiles <= clusters_at_once<NT, kGated>(2 * ranks)) ranks *= 2;
+  return ranks;
+}
+
 template <typename T, int NT, bool kGated>
 int launch_rows(const CUtensorMap& x, const CUtensorMap& w, const Args& a, cudaStream_t st) {
   using F = Few<NT, kGated>;
@@ -742,9 +777,7 @@ int launch_rows(const CUtensorMap& x, const CUtensorMap& w, const Args& a, cudaS
   const int64_t n_tiles = (a.width + kBM - 1) / kBM, slots = F::kCtas * (int64_t)sm_count_of_current_device();
   const int64_t tiles = (a.starts == nullptr ? (a.M + NT - 1) / NT : a.M / NT + (a.groups < a.M ? a.groups : a.M)) * n_tiles;
   ATMA_REQUIRE(tiles < INT32_MAX / 2, "linear_fp8: too many tiles");
-  int ranks = 1;                            // CTAs that share a tile, four blocks each at least
-  if (a.starts == nullptr)
-    while (ranks < 8 && 2 * ranks * tiles <= slots && 4 * 2 * ranks <= a.kb) ranks *= 2;
+  const int ranks = a.starts == nullptr ? ranks_of<NT, kGated>(tiles, a.kb) : 1;
   cudaLaunchAttribute attrs[2];
   attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;              // see early.cuh
   attrs[1].val.programmaticStreamSerializationAllowed = 1;
@@ -757,21 +790,24 @@ int launch_rows(const CUtensorMap& x, const CUtensorMap& w, const Args& a, cudaS
   return launch_status("linear_fp8 (few rows)");
 }
 
-// Which kernel, by a group's rows if all have as many.  The pair kernel reads a weight once for 256 rows, but a pair walks all of K by itself:
-// `chain` blocks one behind another, 5.6 us and 0.4 a block where the weights are in time.  Few rows are bound by the weights, or share K.
-// Either one, us, few rows / many rows:
-//   one weight 8192 x 2048 (chain 16)   64 rows 11.9 / 12.4   80 rows 13.6 / 12.4;   4096 x 4096 (32)   80 rows 13.1 / 18.2
-//   gated, 2 x 4096 x 2048 (16)         24 rows 13.8 / 14.2   40 rows 15.2 / 13.0;   2 x 1024 x 8192 (64)   80 rows 25.7 / 30.6
+// Which kernel, by a group's rows if all have as many.  The pair kernel reads a weight once for 256 rows, but a pair walks all of K by itself,
+// 5.6 us and 0.39 a block; few rows are bound by the weights, and share K: about 7.5 us and 0.58 a block, gated 14 and 0.7 (reading sums
+// from one another and a barrier for every token's scale).  Chains of blocks of one weight are compared by that, experts' rows by what was
+// measured, us, few rows / many rows:
+//   8192 x 2048   64 rows 11.9 / 12.4   80 rows 13.6 / 12.4;   4096 x 4096   128 rows 13.3 / 18.3   512 rows 23.5 / 18.5;
+//   2048 x 8192   256 rows 17.4 / 28.5   512 rows 26.1 / 29.2;   gated 4096 x 2048   40 rows 15.2 / 13.0;   gated 1024 x 8192   256 rows 24.1 / 29.4
 //   64 experts of 2 x 1024 x 2048, the whole feed-forward   32 rows each 105 / 117   48 119 / 119   64 141 / 129   125 203 / 156;
 //   its second product   48 119 / 130   64 141 / 144   96 174 / 165
 template <bool kGated>
 bool many_rows(const Args& a, int each) {
-  const int pairs = sm_count_of_current_device() / 2, wide = kGated ? 128 : 256;
-  const int64_t tiles = (int64_t)a.groups * ((each + 255) / 256) * ((a.width + wide - 1) / wide), turns = (tiles + pairs - 1) / pairs, chain = turns * a.kb;
-  if (each > 128) return true;
-  const bool spread = a.starts != nullptr || turns > 1;      // weights come over all SMs either way
-  if (kGated) return (each > 48 && spread) || (each >= 32 && chain <= 32);
-  return each > 64 && (spread || chain <= 20);
+  if (a.starts != nullptr) return each > (kGated ? 48 : 64);
+  if (each <= 32) return false;
+  auto over = [](int64_t n, int64_t by) { return (n + by - 1) / by; };
+  const int64_t sms = sm_count_of_current_device(), tiles = over(a.M, 64) * over(a.width, 128);
+  const int64_t pair = over(over(a.M, 256) * over(a.width, kGated ? 128 : 256), sms / 2) * a.kb;
+  const int ranks = ranks_of<64, kGated>(tiles, a.kb);
+  const int64_t few = over(tiles * ranks, Few<64, kGated>::kCtas * sms) * over(a.kb, ranks);
+  return kGated ? 10 * pair <= 18 * few + 200 : 10 * pair <= 15 * few + 50;
 }
 
 template <typename T, bool kGated>

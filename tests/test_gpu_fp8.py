@@ -276,7 +276,8 @@ def test_a_row_does_not_depend_on_its_neighbours(M, K):
     assert torch.equal(a.scales[p], b.scales) and torch.equal(a.values.view(torch.uint8)[p], b.values.view(torch.uint8))
 
 
-@pytest.mark.parametrize("M, N, K", [(31, 300, 700), (32, 300, 700), (33, 130, 4224), (65, 520, 2560), (65, 520, 2688), (100, 19000, 200), (50, 9500, 136)])
+@pytest.mark.parametrize("M, N, K", [(31, 300, 700), (32, 300, 700), (33, 130, 4224), (65, 520, 2560), (65, 520, 2688), (100, 19000, 200), (50, 9500, 136),
+                                     (200, 130, 8192), (257, 256, 4104), (400, 128, 4096)])
 def test_products_on_both_sides_of_the_choice_of_kernels(M, N, K):
     test_linear_fp8(M, N, K, torch.float32)
     test_gelu_gated_linear_fp8(M, N // 2, K)
