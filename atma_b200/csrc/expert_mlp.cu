@@ -11,21 +11,19 @@ int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 struct Parts { int64_t rows, row_scales, act, act_scales, y, all; };             // offsets in the scratch memory, bytes
 
-// Experts' results before they are summed: fp32 where that is little (1 us of 124 with 512 tokens, 8 of 64 experts, 2048 / 1024), else in the
-// activation type.  A bf16 sum's error has a 2-norm of 2.3e-3 with that rounding and of 1.7e-3 without; fp32 takes 142 us instead of 130 with
-// 1000 tokens, 695 instead of 602 with 8192.
-constexpr int64_t kWideBytes = 32 << 20;
-bool wide_results(int64_t rows, int width, int dtype) { return dtype == ATMA_F32 || rows * width * 4 <= kWideBytes; }
+// Experts' results are fp32 until they are summed, however many there are, so that the type of out is the only rounding behind the products
+// and a token's precision does not go by the tokens beside it.  (In bf16 a bf16 sum's error has a 2-norm of 2.3e-3 instead of 1.7e-3, for half of
+// the bytes between the two kernels: 8192 tokens, 8 of 64 experts, 2048 / 1024, 682 us instead of 767.)
 
 // Values of 128 bytes more than a row's are never needed: rows start on 16-byte boundaries, parts on 256-byte ones.
-Parts parts_of(int64_t rows, int width, int ff, int size) {
+Parts parts_of(int64_t rows, int width, int ff) {
   Parts p;
   p.rows = 0;
   p.row_scales = round_up(p.rows + rows * round_up(width, 16), 256);
   p.act = round_up(p.row_scales + rows * 4 * ((width + 127) / 128), 256);
   p.act_scales = round_up(p.act + rows * round_up(ff, 16), 256);
   p.y = round_up(p.act_scales + rows * 4 * ((ff + 127) / 128), 256);
-  p.all = p.y + rows * width * size;
+  p.all = p.y + rows * width * (int64_t)sizeof(float);
   return p;
 }
 
@@ -36,7 +34,8 @@ using namespace atma;
 
 extern "C" int64_t atma_expert_mlp_scratch_bytes(int tokens, int copies, int width, int ff, int dtype) {
   if (tokens <= 0 || copies <= 0 || width <= 0 || ff <= 0) return 0;
-  return parts_of((int64_t)tokens * copies, width, ff, wide_results((int64_t)tokens * copies, width, dtype) ? 4 : 2).all;
+  (void)dtype;                              // results between the kernels have one type, whatever out's is
+  return parts_of((int64_t)tokens * copies, width, ff).all;
 }
 
 extern "C" int atma_expert_mlp(const atma_expert_args* args, void* scratch, void* stream) {
@@ -49,8 +48,7 @@ extern "C" int atma_expert_mlp(const atma_expert_args* args, void* scratch, void
   ATMA_REQUIRE(scratch != nullptr && (reinterpret_cast<uintptr_t>(scratch) & 255) == 0, "expert_mlp: scratch memory must be 256-byte aligned");
   ATMA_REQUIRE(a.place != nullptr && a.starts != nullptr && a.weights != nullptr && a.out != nullptr, "expert_mlp: null tensors");
   const int rows = a.tokens * a.copies;
-  const bool wide = wide_results(rows, a.width, a.dtype);
-  const Parts p = parts_of(rows, a.width, a.ff, wide ? 4 : 2);
+  const Parts p = parts_of(rows, a.width, a.ff);
   uint8_t* s = static_cast<uint8_t*>(scratch);
   const int64_t x_rs = round_up(a.width, 16), act_rs = round_up(a.ff, 16);
   float *row_scales = reinterpret_cast<float*>(s + p.row_scales), *act_scales = reinterpret_cast<float*>(s + p.act_scales);
@@ -61,8 +59,8 @@ extern "C" int atma_expert_mlp(const atma_expert_args* args, void* scratch, void
   rc = atma_linear_fp8(&up, stream);
   if (rc != ATMA_OK) return rc;
   const atma_fp8_args down = {s + p.act, act_rs, act_scales, rows, a.w_down, a.w_down_rs, a.w_down_scales, s + p.y, a.width, nullptr, 0,
-                              a.starts, rows, a.width, a.ff, a.experts, 0, wide ? ATMA_F32 : ATMA_BF16};
+                              a.starts, rows, a.width, a.ff, a.experts, 0, ATMA_F32};
   rc = atma_linear_fp8(&down, stream);
   if (rc != ATMA_OK) return rc;
-  return combine_experts(s + p.y, wide, a.place, a.weights, a.add, a.out, a.tokens, a.copies, a.width, a.dtype, (cudaStream_t)stream);
+  return combine_experts(s + p.y, true, a.place, a.weights, a.add, a.out, a.tokens, a.copies, a.width, a.dtype, (cudaStream_t)stream);
 }

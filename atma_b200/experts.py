@@ -85,7 +85,7 @@ def expert_mlp(x, w_gate_up, w_down, routes, add=None, dtype=torch.bfloat16):
     """Gelu-gated feed-forwards of the tokens' experts, weighted and summed: sum over j of weights[t, j] * down(gelu_tanh(gate x_t) * up x_t).
     x: Fp8Rows (tokens, width); w_gate_up (experts, 2, ff, width), w_down (experts, width, ff): Fp8Weight; the activations between them go
     to 8 bits like any rows.  ``add`` (tokens, width) is added.  Returns (tokens, width) in ``dtype``, bfloat16 or float32; the sum
-    is fp32, and so is what is summed, or in ``dtype`` where fp32 would be more than 32 MB."""
+    is fp32, and so is what is summed."""
     if not isinstance(x, Fp8Rows) or not isinstance(w_gate_up, Fp8Weight) or not isinstance(w_down, Fp8Weight) or not isinstance(routes, Routes):
         raise ValueError("expert_mlp takes Fp8Rows, two Fp8Weights and Routes")
     (tokens, width), (chosen, top_k), experts = x.values.shape, routes.ids.shape, routes.experts

@@ -198,7 +198,7 @@ int atma_combine_experts(const void* y, const int32_t* place, const float* weigh
 /* Experts' gelu-gated feed-forwards in 8 bits, weighted and summed: out[t] = add[t] (NULL = 0) + sum over j of weights[t][j]
  * down_e(gelu_tanh(gate_e x_t) * up_e x_t), e the expert of pair (t, j), for pairs ordered as atma_route_experts does.
  * x (tokens, width) in 8 bits; w_gate_up [experts][2][ff] rows of width, w_down [experts][width] rows of ff; add and out
- * (tokens, width) dense in dtype.  Sums are fp32; an expert's results are too before they are summed, or in dtype where fp32 would be more than 32 MB.
+ * (tokens, width) dense in dtype.  Sums are fp32, and so are an expert's results before they are summed.
  * scratch: atma_expert_mlp_scratch_bytes(), 256-byte aligned. */
 typedef struct {
   const void* x; int64_t x_rs; const float* x_scales; int64_t xs_bs;

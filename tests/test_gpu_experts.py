@@ -331,3 +331,13 @@ def test_norm_routing_and_experts_in_a_graph():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want[0]) and torch.equal(total, want[1])
+
+
+def test_expert_mlp_rounds_large_sums_once():
+    """As many tokens as there may be: what is summed, here 35 MB of it, is fp32 for a 16-bit result too."""
+    e, f = routing(), ops()
+    w_in, w_out = weight8((4, 2, 128, 256), 1)[0], weight8((4, 256, 128), 2)[0]
+    x = f.quantize_rows(rand((17000, 256), 1, dtype=torch.bfloat16).cuda())
+    routes = e.route_experts(rand((17000, 4), 3).cuda(), 2)
+    fine = e.expert_mlp(x, w_in, w_out, routes, dtype=torch.float32)
+    assert torch.equal(e.expert_mlp(x, w_in, w_out, routes), fine.bfloat16())
