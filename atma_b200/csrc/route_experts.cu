@@ -33,6 +33,12 @@ constexpr int kMaxExperts = 512;
 // reciprocal and the sum with the bias, 2.5e-7 + 6e-8 |key|.  Softmax: up to 22 roundings of the sum, which all keys share, as well.
 constexpr float kKeyError = 4e-6f, kSigmoidError = 1e-6f;
 
+// How far the sum of a group's two best keys may be off: half of `error` for either key and |key| + 1, not for their sum, where keys of
+// opposite signs cancel.  The sum's own rounding is in what kSigmoidError and kKeyError leave of every key.  One key: second = 0.
+__device__ __forceinline__ float group_reach(float best, float second, float error) {
+  return fmaf(.5f * error, fabsf(best), fmaf(.5f * error, fabsf(second), error));
+}
+
 struct RouteArgs {
   const float* logits; int64_t l_rs;
   const float* bias;
@@ -107,6 +113,8 @@ __device__ __forceinline__ bool keep_groups(typename Ordered<F>::type (&key)[V],
   using U = typename Ordered<F>::type;
   const int lane = threadIdx.x & 31, size = a.experts / a.groups;
   U mine[2] = {0, 0};                                        // keys of groups `lane` and `lane + 32`
+  float reach[2] = {0.f, 0.f};                               // fp32: how far they may be off; nothing where a key is infinite
+  bool settled = true;
   for (int g = 0; g < a.groups; ++g) {
     U best = 0, second = 0;
 #pragma unroll
@@ -121,22 +129,29 @@ __device__ __forceinline__ bool keep_groups(typename Ordered<F>::type (&key)[V],
     // a group of one expert has no second; inf and -inf are inf
     const F sum = next == 0 || value_of(most) == F(INFINITY) ? value_of(most) : value_of(most) + value_of(next);
     if (lane == (g & 31)) mine[g >> 5] = ordered(sum);
+    if constexpr (std::is_same<F, float>::value) {
+      const float r = group_reach(value_of(most), next == 0 ? 0.f : value_of(next), kKeyError);
+      if (fabsf(sum) <= FLT_MAX) {
+        if (lane == (g & 31)) reach[g >> 5] = r;
+      } else if (r <= FLT_MAX) {                             // finite keys whose sum is not
+        settled = false;
+      }
+    }
   }
   uint64_t left = 0;
-  U last = 0;
-  bool settled = true;
+  float lowest = INFINITY;                                   // what a group that stays has at least
   for (int n = 0; n <= a.top_groups && n < a.groups; ++n) {
-    const U most = warp_most(mine[0] > mine[1] ? mine[0] : mine[1]);
-    const uint32_t low = __ballot_sync(0xffffffffu, mine[0] == most), high = __ballot_sync(0xffffffffu, mine[1] == most);
-    const int g = low ? __ffs(low) - 1 : 31 + __ffs(high);
-    if (n == a.top_groups) {                                 // the best one that goes: too near to the last that stays?
+    if (n == a.top_groups) {                                 // the others go: may one of them have as much?
       if constexpr (std::is_same<F, float>::value) {
-        const float p = value_of(last), q = value_of(most);
-        settled = p - q > 2.f * kKeyError * (fabsf(p) + 1.f);
+        const float highest = fmaxf(mine[0] == 0 ? -INFINITY : value_of(mine[0]) + reach[0], mine[1] == 0 ? -INFINITY : value_of(mine[1]) + reach[1]);
+        settled = settled && lowest > value_of(warp_most(ordered(highest)));
       }
       break;
     }
-    last = most;
+    const U most = warp_most(mine[0] > mine[1] ? mine[0] : mine[1]);
+    const uint32_t low = __ballot_sync(0xffffffffu, mine[0] == most), high = __ballot_sync(0xffffffffu, mine[1] == most);
+    const int g = low ? __ffs(low) - 1 : 31 + __ffs(high);
+    if constexpr (std::is_same<F, float>::value) lowest = fminf(lowest, value_of(most) - __shfl_sync(0xffffffffu, reach[g >> 5], g & 31));
     left |= 1ull << g;
     if (lane == (g & 31)) mine[g >> 5] = 0;
   }
@@ -344,16 +359,17 @@ __device__ __forceinline__ bool choose_fast(const float (&z)[V], const float (&b
       best = fmaxf(best, b);
     }
     const float both = second == -INFINITY ? best : best + second;
+    const float reach = group_reach(best, second == -INFINITY ? 0.f : second, width);
     int above = 0;                          // groups that are better than this lane's
-    float nearest = INFINITY;
+    float nearest = INFINITY;               // of the distances from another one, less what that one may be off by
 #pragma unroll 4
     for (int from = 0; from < a.groups * lanes; from += lanes) {
-      const float other = __shfl_sync(0xffffffffu, both, from);
+      const float other = __shfl_sync(0xffffffffu, both, from), its = __shfl_sync(0xffffffffu, reach, from);
       above += other > both;
-      nearest = fminf(nearest, from == mine ? INFINITY : fabsf(other - both));
+      nearest = fminf(nearest, from == mine ? INFINITY : fabsf(other - both) - its);
     }
     // two infinities are as near as can be
-    const bool settled = (nearest > 2.f * width * (fabsf(both) + 1.f) && fabsf(both) <= FLT_MAX) || lane >= a.groups * lanes;
+    const bool settled = (nearest > reach && fabsf(both) <= FLT_MAX) || lane >= a.groups * lanes;
     out = above >= a.top_groups;
     if (!__all_sync(0xffffffffu, settled)) out = group_goes_in_64<V>(row, e0, m, a);
   }

@@ -341,3 +341,23 @@ def test_expert_mlp_rounds_large_sums_once():
     routes = e.route_experts(rand((17000, 4), 3).cuda(), 2)
     fine = e.expert_mlp(x, w_in, w_out, routes, dtype=torch.float32)
     assert torch.equal(e.expert_mlp(x, w_in, w_out, routes), fine.bfloat16())
+
+
+def test_route_experts_groups_whose_keys_cancel_by_hand():
+    """Sums of 0.980572 and 0.980638 of keys around 1e5 and -1e5: fp32 ones are 0.984375 and 0.9765625."""
+    x, bias = torch.tensor([[0.07926305, -0.15725687, -0.8928827, 0.80069155]]), torch.tensor([1e5, -1e5, 1e5, -1e5])
+    r = routing().route_experts(x.cuda(), 2, score="sigmoid", bias=bias.cuda(), groups=2, top_groups=1)
+    assert r.ids.tolist() == O.route(x, 2, "sigmoid", bias, 2, 1)[0] == [[2, 3]]
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("most", [16.0, 64.0, 1e3, 1e4, 1e5, 1e6, 3e38])
+@pytest.mark.parametrize("experts, groups, top_groups, k", [(4, 2, 1, 2), (64, 8, 3, 4), (24, 8, 3, 4), (160, 8, 3, 6), (128, 64, 7, 9)])
+def test_route_experts_groups_whose_keys_cancel(experts, groups, top_groups, k, most, score):
+    """The two best keys of every group are near a bias and near its opposite: their sum says nothing of what they are off by."""
+    size = experts // groups
+    bias = torch.full((groups, size), -1.125 * most if most < 1e38 else -math.inf)
+    bias[:, 0], bias[:, 1] = most, -most
+    x, bias = rand((600, experts), 11), bias.flatten()
+    r = routing().route_experts(x.cuda(), k, score=score, bias=bias.cuda(), groups=groups, top_groups=top_groups)
+    assert r.ids.tolist() == O.route(x, k, score, bias, groups, top_groups)[0]
