@@ -7,7 +7,8 @@
 // A choice is only as good as the difference between the keys that it turns on, and fp32 keys are off by some 1e-7.  So a warp takes
 // a token in fp32 first, and where two neighbours among the sorted best (and the first one left out, and the groups likewise) are
 // nearer to one another than their errors can reach, those are decided again with keys in fp64.  Without a bias and groups both scores
-// grow with the logit, which is then the key itself and exact.
+// grow with the logit, which is then the key itself and exact.  Weights are fp32 scores over their sum, and fp64 ones where the chosen scores
+// are below what fp32 holds: sigmoids of logits below -87, softmax beside a far larger logit that a bias or its group keeps out.
 //
 // Bound by instructions: 16384 tokens of 256 experts in 8 groups, top 8, 28 us and 9 for the order (18 MB: 2.8); 75 and 15 with a scan of the
 // lane's keys in every round and whole tokens again in fp64, which held up their CTAs by 10 us each.
@@ -77,6 +78,13 @@ template <> struct Ordered<double> { using type = uint64_t; };
 __device__ __forceinline__ float exp_of(float x) { return expf(x); }
 __device__ __forceinline__ double exp_of(double x) { return exp(x); }
 
+// The exponential is 1 at most: e^-z has no fp32 value below z = -88, where the result still has one.
+__device__ __forceinline__ float sigmoid_of(float z) {
+  const float e = expf(-fabsf(z));
+  return (z < 0.f ? e : 1.f) / (1.f + e);
+}
+__device__ __forceinline__ double sigmoid_of(double z) { return 1. / (1. + exp(-z)); }
+
 template <typename F>
 __device__ __forceinline__ F warp_add(F v) {
 #pragma unroll
@@ -89,7 +97,7 @@ template <typename F, int V>
 __device__ __forceinline__ void scores_of(const float (&z)[V], int e0, int experts, bool sigmoid, F (&s)[V]) {
   if (sigmoid) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) s[v] = F(1) / (F(1) + exp_of(-F(z[v])));
+    for (int v = 0; v < V; ++v) s[v] = sigmoid_of(F(z[v]));
     return;
   }
   float m = -FLT_MAX;
@@ -250,7 +258,7 @@ __device__ __forceinline__ void sort_words(uint32_t (&w)[V]) {
 __device__ __forceinline__ double key_in_64(const float* row, int e, float m, double total, const RouteArgs& a) {
   const double z = logit_of(row[e]);
   if (a.bias == nullptr && a.groups == 1) return z;
-  const double s = a.sigmoid ? 1. / (1. + exp(-z)) : exp(z - (double)m) / total;
+  const double s = a.sigmoid ? sigmoid_of(z) : exp(z - (double)m) / total;
   if (a.bias == nullptr) return s;
   const float b = a.bias[e];
   return s + (isnan(b) ? -INFINITY : b);
@@ -261,6 +269,22 @@ __device__ __forceinline__ double total_in_64(const float* row, float m, const R
 #pragma unroll 1
     for (int i = threadIdx.x & 31; i < a.experts; i += 32) total += exp((double)logit_of(row[i]) - (double)m);
   return warp_add(total);
+}
+
+// Weights of a token whose chosen scores are not, or hardly, fp32 values: the scores over their sum in fp64 (softmax: the sum over all experts
+// is in both and left out), zero where that sum is.  Two choices a lane, where they are used.
+struct Two { float v[2]; };
+__device__ __noinline__ Two weights_in_64(const float* row, int e0, int e1, bool used0, bool used1, const RouteArgs& a) {
+  float m = -FLT_MAX;
+  if (!a.sigmoid) {
+#pragma unroll 1
+    for (int i = threadIdx.x & 31; i < a.experts; i += 32) m = fmaxf(m, logit_of(row[i]));
+    m = value_of(warp_most(ordered(m)));
+  }
+  const double x = logit_of(row[e0]), y = logit_of(row[e1]);
+  const double s = !used0 ? 0. : a.sigmoid ? sigmoid_of(x) : exp(x - (double)m), t = !used1 ? 0. : a.sigmoid ? sigmoid_of(y) : exp(y - (double)m);
+  const double sum = warp_add(s + t);
+  return {{sum > 0. ? (float)(s / sum) : 0.f, sum > 0. ? (float)(t / sum) : 0.f}};
 }
 
 // Of n taken experts, one a lane, how many have a larger key, in fp64.  Out of line, like the next one: one token in some dozens comes
@@ -415,7 +439,7 @@ __device__ __forceinline__ bool choose_fast(const float (&z)[V], const float (&b
   const float x = logit_of(row[e]);
   *id = e;
   *rank = lane < n ? lane : 32;
-  *score = a.sigmoid ? 1.f / (1.f + expf(-x)) : expf(x - m) / sum;
+  *score = a.sigmoid ? sigmoid_of(x) : expf(x - m) / sum;
   if (near) *rank = rank_in_64(row, e, n, m, a);             // the same for all lanes
   return true;
 }
@@ -532,9 +556,16 @@ route_experts_kernel(const __grid_constant__ RouteArgs a) {
       score[0] = c.score[0]; score[1] = c.score[1];
     }
     if (a.renormalize) {
-      const float sum = warp_sum((rank[0] < a.k ? score[0] : 0.f) + (rank[1] < a.k ? score[1] : 0.f));
+      const bool used[2] = {rank[0] < a.k, rank[1] < a.k};
+      const float sum = warp_sum((used[0] ? score[0] : 0.f) + (used[1] ? score[1] : 0.f));
+      // a score below fp32's least normal value has fewer bits, or none; over a sum from 2^-20 on that is less than 2^-129 of a weight
+      if (sum < 0x1p-20f && __any_sync(0xffffffffu, (used[0] && score[0] < FLT_MIN) || (used[1] && score[1] < FLT_MIN))) {
+        const Two w = weights_in_64(row, id[0], id[1], used[0], used[1], a);
+        score[0] = w.v[0]; score[1] = w.v[1];
+      } else {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) score[i] = sum > 0.f ? score[i] / sum : 0.f;
+        for (int i = 0; i < 2; ++i) score[i] /= sum;
+      }
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)

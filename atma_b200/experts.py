@@ -46,7 +46,7 @@ def route_experts(logits, top_k, *, score="softmax", bias=None, groups=1, top_gr
     (experts,) float32, weights by the scores alone.  ``groups``: of so many groups of neighbouring experts only ``top_groups`` are
     looked at, those with the largest sum of their two best (None: all).  ``renormalize``: a token's weights are divided by their sum (zero where that is
     zero); ``scale`` multiplies them.  Equal ones: the lower index first.  NaN and -inf count as the least finite logit, inf as the
-    largest; a choice is decided as in 64-bit arithmetic."""
+    largest; a choice is decided as in 64-bit arithmetic, and scores too small for fp32 are divided in it."""
     here, shape = _here(logits, bias), logits.shape
     if len(shape) != 2 or not logits.dtype.is_floating_point:
         raise ValueError("logits must be a (tokens, experts) matrix")

@@ -179,7 +179,7 @@ int atma_linear_fp8(const atma_fp8_args* args, void* stream);
 /* Experts of tokens.  score = sigmoid(logit) or softmax(logits), key = score + bias (NULL = none); of `groups` groups of
  * neighbouring experts the top_groups with the largest sum of their two largest keys stay; ids [tokens][k]: the k largest
  * keys of those, falling, lower indices first among equal ones; weights [tokens][k]: their scores, divided by their sum
- * (renormalize; zero where that is zero), times scale.  NaN and -infinity count as the least finite logit, infinity as
+ * (renormalize; zero where that is zero in 64 bits), times scale.  NaN and -infinity count as the least finite logit, infinity as
  * the largest.  order [tokens * k]: token * k + choice of every pair, by expert, then by itself; place: its inverse;
  * starts [experts + 1]: where every expert's pairs begin.  scratch: atma_route_scratch_ints() words. */
 int atma_route_experts(const float* logits, int64_t l_rs, const float* bias, int32_t* ids, float* weights, int32_t* order,

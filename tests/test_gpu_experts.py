@@ -361,3 +361,40 @@ def test_route_experts_groups_whose_keys_cancel(experts, groups, top_groups, k, 
     x, bias = rand((600, experts), 11), bias.flatten()
     r = routing().route_experts(x.cuda(), k, score=score, bias=bias.cuda(), groups=groups, top_groups=top_groups)
     assert r.ids.tolist() == O.route(x, k, score, bias, groups, top_groups)[0]
+
+
+# experts, k, options: lanes with one and with several experts, groups of no whole lanes, more choices than lanes
+SMALL_SCORES = [(4, 2, {}), (64, 2, {}), (64, 7, dict(groups=8, top_groups=6)), (64, 40, {}), (24, 7, dict(groups=8, top_groups=7)), (300, 2, {}), (300, 40, {})]
+
+
+def check_weights(r, logits, k, score, bias=None, **kw):
+    """128 u as above, u |z - max| of the exponent's argument in a score and in the sum; what fp32 has no bits for."""
+    ids, weights = O.route(logits, k, score, bias, **kw)
+    assert r.ids.tolist() == ids
+    w = torch.tensor(weights, dtype=torch.float64)
+    span = float(logits.max() - logits.min()) if score == "softmax" else 0
+    assert ((r.weights.cpu().double() - w).abs() <= (128 + 2 * span) * U * w + 2.0 ** -129).all()
+    return w
+
+
+@pytest.mark.parametrize("experts, k, kw", SMALL_SCORES)
+@pytest.mark.parametrize("low, high", [(-98, -95), (-90, -80), (-105, -87), (-300, -90), (-120, -20), (-120, 3)])
+def test_route_experts_weights_of_sigmoids_that_fp32_does_not_hold(experts, k, kw, low, high):
+    x = low + (high - low) * torch.rand(60, experts, generator=torch.Generator().manual_seed(1))
+    r = routing().route_experts(x.cuda(), k, score="sigmoid", **kw)
+    w = check_weights(r, x, k, "sigmoid", **kw)
+    assert ((w.sum(1) - 1).abs() < 1e-12).all()
+    check_weights(routing().route_experts(x.cuda(), k, score="sigmoid", renormalize=False, **kw), x, k, "sigmoid", renormalize=False, **kw)
+
+
+@pytest.mark.parametrize("experts, k, kw", SMALL_SCORES)
+@pytest.mark.parametrize("gap", [60, 85, 95, 110, 200, 600])
+def test_route_experts_weights_beside_a_larger_logit_that_is_kept_out(experts, k, kw, gap):
+    x, bias = 3 * rand((60, experts), 5), torch.zeros(experts)
+    x[:, 1] = gap
+    bias[1] = -math.inf
+    check_weights(routing().route_experts(x.cuda(), k, bias=bias.cuda(), **kw), x, k, "softmax", bias, **kw)
+    if "groups" in kw:                                       # by its group
+        bias = torch.zeros(experts)
+        bias[:experts // kw["groups"]] = -3.0
+        check_weights(routing().route_experts(x.cuda(), k, bias=bias.cuda(), **kw), x, k, "softmax", bias, **kw)
