@@ -20,7 +20,8 @@ MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 512, 64, 64
 class Routes:
     """Where tokens go.  ids, weights (tokens, top_k): experts (int32) and their weights (float32), the best first.  A pair
     token * top_k + choice is a row of the experts' products: order[row] = pair (rows by expert, then by pair), place[pair] = row,
-    and expert e's rows are starts[e] .. starts[e + 1] - 1 (all int32)."""
+    and expert e's rows are starts[e] .. starts[e + 1] - 1 (all int32).  weights may be replaced by others of the same shape; ids are what the
+    places were made from."""
 
     __slots__ = ("ids", "weights", "experts", "_plan")
 
@@ -95,13 +96,16 @@ def expert_mlp(x, w_gate_up, w_down, routes, add=None, dtype=torch.bfloat16):
                          f"{tuple(routes.ids.shape)} choices of {experts} experts")
     if routes.weights.shape != routes.ids.shape or routes.weights.dtype is not torch.float32 or not routes.weights.is_contiguous():
         raise ValueError("the routes' weights must be (tokens, top_k) float32, contiguous")
+    plan = routes._plan                          # other ids than route_experts gave have other places: rows would be written behind the scratch memory
+    if plan.shape != (2 * tokens * top_k + experts + 1,) or plan.dtype is not torch.int32 or not plan.is_contiguous():
+        raise ValueError(f"the routes' places are not those of {tokens} tokens with {top_k} of {experts} experts: another choice takes another call of route_experts")
     if dtype not in _TYPES or add is not None and (add.shape != (tokens, width) or add.dtype is not dtype or not add.is_contiguous()):
         raise ValueError("bfloat16 or float32, add contiguous in the same type")
-    here, dev = _here(x.values, w_gate_up.values, w_down.values, routes._plan, routes.weights, add), x.values.device
+    here, dev = _here(x.values, w_gate_up.values, w_down.values, plan, routes.weights, add), x.values.device
     lib, code = _lib.load_decoder(), _lib.DTYPE_CODE[dtype]
     out = _new((tokens, width), (width, 1), device=dev, dtype=dtype)
     scratch = _new((lib.atma_expert_mlp_scratch_bytes(tokens, top_k, width, ff, code),), (1,), device=dev, dtype=torch.uint8)
-    place = routes._plan.data_ptr() + 4 * tokens * top_k
+    place = plan.data_ptr() + 4 * tokens * top_k
     a = _lib.ExpertArgs(x.values.data_ptr(), x.row_stride, x.scales.data_ptr(), x.scale_stride, w_gate_up.values.data_ptr(), w_gate_up.row_stride,
                         w_gate_up.scales.data_ptr(), w_down.values.data_ptr(), w_down.row_stride, w_down.scales.data_ptr(), place, place + 4 * tokens * top_k,
                         routes.weights.data_ptr(), None if add is None else add.data_ptr(), out.data_ptr(), tokens, top_k, experts, width, ff, code)

@@ -142,6 +142,22 @@ def test_routes_with_other_weights(anywhere):
             e.expert_mlp(r, *stack, routes)
 
 
+def test_routes_with_other_choices_are_refused(anywhere):
+    """Places go with the choices that they were made for: fewer, more or other ones would send rows behind the scratch memory."""
+    f, e = anywhere
+    r, stack = f.Fp8Rows(torch.zeros(4, 256, dtype=f.E4M3), torch.zeros(4, 2)), (f.Fp8Weight.of(torch.zeros(6, 2, 32, 256)), f.Fp8Weight.of(torch.zeros(6, 256, 32)))
+    routes = lambda k, plan, tokens=4: e.Routes(torch.zeros(tokens, k, dtype=torch.int32), torch.zeros(tokens, k), 6, plan)
+    two = torch.zeros(2 * 4 * 2 + 7, dtype=torch.int32)
+    with pytest.raises(AssertionError, match="came through"):
+        e.expert_mlp(r, *stack, routes(2, two))
+    some = routes(2, two)
+    some.ids, some.weights = some.ids[:, :1].contiguous(), some.weights[:, :1].contiguous()               # the best one alone
+    for x, bad in ((r, some), (r, routes(3, two)), (r, routes(1, two)), (r, routes(2, two.long())), (r, routes(2, two[None])), (r, routes(2, two[:22])),
+                   (r, routes(2, torch.zeros(46, dtype=torch.int32)[::2])), (r[:3], routes(2, two, 3))):
+        with pytest.raises(ValueError, match="places"):
+            e.expert_mlp(x, *stack, bad)
+
+
 @pytest.fixture(scope="module")
 def lib():
     from atma_b200 import _lib
