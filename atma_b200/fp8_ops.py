@@ -43,6 +43,12 @@ def _apart(out, *inputs):
             raise ValueError("results must not overlap what is read")
 
 
+def _own(out):
+    """Refuses results into a copy: the memory that the caller named would keep what it has."""
+    if out.copied:
+        raise ValueError("out must be rows that start on 16-byte boundaries with scales that lie block by block; these were copied")
+
+
 def _stride(width):
     """Bytes between rows that start on 16-byte boundaries."""
     return width + -width % 16
@@ -76,9 +82,9 @@ def _row_stride(values):
 
 class Fp8Rows:
     """Rows in 8 bits: ``values`` (rows, width) float8_e4m3fn, ``scales`` (rows, blocks) float32.  Rows that do not start on 16-byte
-    boundaries and scales that do not lie block by block (stride 1 along the rows) are copied."""
+    boundaries and scales that do not lie block by block (stride 1 along the rows) are copied, and such rows take no results."""
 
-    __slots__ = ("values", "scales", "row_stride", "scale_stride")
+    __slots__ = ("values", "scales", "row_stride", "scale_stride", "copied")
 
     def __init__(self, values, scales):
         shape = values.shape
@@ -87,17 +93,18 @@ class Fp8Rows:
         if scales.get_device() != values.get_device():
             raise ValueError("values and scales must be on one device")
         (rows, width), (step, unit) = shape, values.stride()
+        self.copied = False
         if rows < 2 or unit != 1 or step < width or step % 16 or values.data_ptr() % 16:
             step = _row_stride(values)
             if step is None:
                 values = _storage(shape[:1], width, values.device).copy_(values)
-                step = _stride(width)
+                step, self.copied = _stride(width), rows > 0
         self.row_stride = step
         along, step = scales.stride()
         if width <= BLOCK:                       # one block: its stride is not used
             step = rows
         if rows > 1 and along != 1 or step < rows:
-            scales, step = scales.t().contiguous().t(), rows
+            scales, step, self.copied = scales.t().contiguous().t(), rows, True
         self.values, self.scales, self.scale_stride = values, scales, step if step > 0 else 1      # words between neighbouring blocks' scales
 
     @property
@@ -177,6 +184,7 @@ class Fp8Weight:
 def empty_rows(rows, width, device):
     """Fp8Rows (rows, width) in new memory, not filled."""
     r = Fp8Rows.__new__(Fp8Rows)
+    r.copied = False
     r.row_stride, r.scale_stride = rs, bs = width + -width % 16, rows if rows else 1
     r.values = _new((rows, width), (rs, 1), device=device, dtype=E4M3)
     r.scales = _new((rows, -(-width // BLOCK)), (1, bs), device=device, dtype=torch.float32)
@@ -192,6 +200,7 @@ def quantize_rows(x, out=None):
     if out is not None:
         if out.shape != x.shape:
             raise ValueError(f"out has the shape {tuple(out.shape)}, x {tuple(x.shape)}")
+        _own(out)
         _apart(out.values, x), _apart(out.scales, x)
     if x.stride(1) != 1 and x.shape[1] > 1:
         x = x.contiguous()
@@ -298,6 +307,7 @@ def gelu_gated_linear_fp8(x, weight, out=None):
     if out is not None:
         if out.shape != (x.shape[0], weight.shape[1]):
             raise ValueError(f"out has the shape {tuple(out.shape)}, the result {(x.shape[0], weight.shape[1])}")
+        _own(out)
         for t in (out.values, out.scales):
             _apart(t, x.values, x.scales, weight.values, weight.scales)
     return _product(x, weight, empty_rows(x.shape[0], weight.shape[1], x.values.device) if out is None else out, here)

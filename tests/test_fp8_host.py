@@ -158,6 +158,21 @@ def test_routes_with_other_choices_are_refused(anywhere):
             e.expert_mlp(x, *stack, bad)
 
 
+def test_results_into_rows_that_were_copied_are_refused(anywhere):
+    """Every other row of wider rows: their values lie where they did, their scales do not, and would stay as they were."""
+    f, _ = anywhere
+    big, x = f.Fp8Rows(torch.zeros(8, 256, dtype=f.E4M3), torch.zeros(2, 8).t()), torch.zeros(4, 256)
+    gate, r = f.Fp8Weight.of(torch.zeros(2, 256, 256)), f.Fp8Rows(torch.zeros(4, 256, dtype=f.E4M3), torch.zeros(2, 4).t())
+    for out in (big[::2], f.Fp8Rows(torch.zeros(4, 256, dtype=f.E4M3), torch.zeros(4, 2)), f.Fp8Rows(torch.zeros(4, 257, dtype=f.E4M3)[:, 1:], torch.zeros(2, 4).t())):
+        for call in (lambda: f.quantize_rows(x, out=out), lambda: f.gelu_gated_linear_fp8(r, gate, out=out)):
+            with pytest.raises(ValueError, match="copied"):
+                call()
+    for out in (big[2:6], f.Fp8Rows(torch.zeros(9, 272, dtype=f.E4M3)[::2], torch.zeros(3, 5).t())[:4].columns(0, 256), f.empty_rows(4, 256, "cpu")):
+        assert not out.copied
+        with pytest.raises(AssertionError, match="came through"):
+            f.quantize_rows(x, out=out)
+
+
 @pytest.fixture(scope="module")
 def lib():
     from atma_b200 import _lib
