@@ -15,6 +15,7 @@ from .decoder_ops import _check
 from .fp8_ops import Fp8Rows, Fp8Weight, _here, _new, _stream, _TYPES
 
 MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 512, 64, 64
+_EXACT = (torch.float32, torch.bfloat16, torch.float16)       # what float32, which a choice is made from, holds without rounding
 
 
 class Routes:
@@ -43,14 +44,14 @@ class Routes:
 
 
 def route_experts(logits, top_k, *, score="softmax", bias=None, groups=1, top_groups=None, renormalize=True, scale=1.0):
-    """Experts of tokens by their logits (tokens, experts).  ``score``: "softmax" or "sigmoid"; a choice goes by score + ``bias``
-    (experts,) float32, weights by the scores alone.  ``groups``: of so many groups of neighbouring experts only ``top_groups`` are
+    """Experts of tokens by their logits (tokens, experts), float32 or 16-bit.  ``score``: "softmax" or "sigmoid"; a choice goes by score +
+    ``bias`` (experts,), float32 or 16-bit, weights by the scores alone.  ``groups``: of so many groups of neighbouring experts only ``top_groups`` are
     looked at, those with the largest sum of their two best (None: all).  ``renormalize``: a token's weights are divided by their sum (zero where that is
     zero); ``scale`` multiplies them.  Equal ones: the lower index first.  NaN and -inf count as the least finite logit, inf as the
     largest; a choice is decided as in 64-bit arithmetic, and scores too small for fp32 are divided in it."""
     here, shape = _here(logits, bias), logits.shape
-    if len(shape) != 2 or not logits.dtype.is_floating_point:
-        raise ValueError("logits must be a (tokens, experts) matrix")
+    if len(shape) != 2 or logits.dtype not in _EXACT:
+        raise ValueError("logits must be a (tokens, experts) matrix of float32, bfloat16 or float16")
     (tokens, experts), dev = shape, logits.device
     if top_groups is None:
         top_groups = groups
@@ -64,8 +65,8 @@ def route_experts(logits, top_k, *, score="softmax", bias=None, groups=1, top_gr
     if logits.dtype is not torch.float32 or unit != 1 and experts > 1 or step < experts and tokens > 1:
         logits, step = logits.float().contiguous(), experts
     if bias is not None:
-        if bias.shape != (experts,):
-            raise ValueError(f"bias must have {experts} values, not the shape {tuple(bias.shape)}")
+        if bias.shape != (experts,) or bias.dtype not in _EXACT:
+            raise ValueError(f"bias must have {experts} values of float32, bfloat16 or float16, not the shape {tuple(bias.shape)} of {bias.dtype}")
         if bias.dtype is not torch.float32 or not bias.is_contiguous():
             bias = bias.float().contiguous()
     lib, n, i32 = _lib.load_decoder(), tokens * top_k, torch.int32

@@ -173,6 +173,18 @@ def test_results_into_rows_that_were_copied_are_refused(anywhere):
             f.quantize_rows(x, out=out)
 
 
+def test_routing_refuses_what_fp32_would_round(anywhere):
+    """Logits that differ in 64 bits alone would be equal, and the lower index would win: a choice is as in 64-bit arithmetic or refused."""
+    _, e = anywhere
+    z = torch.zeros(4, 12)
+    for call in (lambda: e.route_experts(z.double(), 2), lambda: e.route_experts(z, 2, bias=z[0].double()), lambda: e.route_experts(z, 2, bias=z[0].long())):
+        with pytest.raises(ValueError, match="float32"):
+            call()
+    for logits, bias in ((z, None), (z.bfloat16(), z[0].half()), (z.half(), z[0].bfloat16())):
+        with pytest.raises(AssertionError, match="came through"):
+            e.route_experts(logits, 2, bias=bias)
+
+
 @pytest.fixture(scope="module")
 def lib():
     from atma_b200 import _lib
