@@ -283,10 +283,13 @@ def _product(x, weight):
 
 def linear(x, weight, out=None, dtype=None):
     """x @ weight.T in the activation dtype: the weight-streaming kernel for up to 16 16-bit rows, ``linear_f32`` for
-    fp32 rows in numbers, cuBLAS otherwise.  Of rows and a weight in 8 bits: ``fp8_ops.linear_fp8`` in ``dtype`` (None: bfloat16)."""
+    fp32 rows in numbers, cuBLAS otherwise.  Of rows and a weight in 8 bits: ``fp8_ops.linear_fp8`` in ``dtype`` (None: bfloat16);
+    other products have the weight's type, and no other ``dtype``."""
     if not isinstance(weight, torch.Tensor):
         from .fp8_ops import linear_fp8
         return linear_fp8(x, weight, out, torch.bfloat16 if dtype is None else dtype)
+    if dtype is not None and dtype is not weight.dtype:
+        raise ValueError(f"a product with a weight in {weight.dtype} is not in {dtype}")
     from .inference_ops import decode_linear, decode_linear_supported
     if decode_linear_supported(x, weight):
         return decode_linear(x, weight, out=out, lib=_lib.load_decoder())

@@ -185,6 +185,15 @@ def test_routing_refuses_what_fp32_would_round(anywhere):
             e.route_experts(logits, 2, bias=bias)
 
 
+def test_linear_refuses_a_type_that_it_would_not_give():
+    from atma_b200 import decoder_ops
+    x, w = torch.zeros(2, 128, dtype=torch.bfloat16), torch.zeros(3, 128, dtype=torch.bfloat16)
+    for dtype in (torch.float32, torch.float16):
+        with pytest.raises(ValueError, match="bfloat16"):
+            decoder_ops.linear(x, w, dtype=dtype)
+    assert decoder_ops.linear(x, w, dtype=torch.bfloat16).dtype == decoder_ops.linear(x, w).dtype == torch.bfloat16
+
+
 @pytest.fixture(scope="module")
 def lib():
     from atma_b200 import _lib
