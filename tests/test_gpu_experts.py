@@ -398,3 +398,46 @@ def test_route_experts_weights_beside_a_larger_logit_that_is_kept_out(experts, k
         bias = torch.zeros(experts)
         bias[:experts // kw["groups"]] = -3.0
         check_weights(routing().route_experts(x.cuda(), k, bias=bias.cuda(), **kw), x, k, "softmax", bias, **kw)
+
+
+@pytest.mark.parametrize("tokens, n, k, width, ff, skew", [
+    (64, 64, 2, 128, 1024, 0),       # 2 rows an expert, 16 tokens wide: 500 gated tiles for 296 CTAs
+    (600, 48, 2, 130, 1024, 0),      # 25 rows, 32 wide: over 400
+    (480, 24, 2, 128, 1100, 0),      # 40 rows, 64 wide, a CTA an SM: 220 and more
+    (760, 24, 2, 128, 1300, 0),      # 63 rows, pairs of SMs: 264 tiles for 74
+    (2400, 3, 1, 130, 2900, 9),      # ten tiles of one expert's rows, which go in bands of eight; the other experts have none
+])
+def test_expert_mlp_where_ctas_take_several_tiles(tokens, n, k, width, ff, skew):
+    e, f = routing(), ops()
+    h = loud(tokens, width, tokens, torch.bfloat16)
+    w_in, in_wide = weight8((n, 2, ff, width), 1)
+    w_out, out_wide = weight8((n, width, ff), 2)
+    logits = rand((tokens, n), 3)
+    logits[:, 0] += skew
+    routes = e.route_experts(logits.cuda(), k, score="sigmoid")
+    y = e.expert_mlp(f.quantize_rows(h.cuda()), w_in, w_out, routes, dtype=torch.float32)
+    want, off, most = O.expert_mlp(O.wide_rows(*O.quantize(h.double())), [in_wide[2 * i:2 * i + 2] for i in range(n)], out_wide, routes.ids.tolist(),
+                                   routes.weights.double().tolist(), product_error(max(width, ff)))
+    off = off + (k + 4) * U * (most + off)                   # as in test_expert_mlp
+    assert ((y.cpu().double() - want).abs() <= off + 1e-40).all()
+    assert off.norm() < 0.03 * want.norm()                   # a tile in another's place would be off by all of it
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tokens, k, D", [(1, 1, 1), (5, 3, 20), (40, 8, 264), (7, 11, 1001)])
+def test_weighted_sum_by_its_c_entry(tokens, k, D, dtype):
+    """atma_combine_experts, for a caller with results of its own: k fmas in fp32 and one rounding."""
+    from atma_b200 import _lib
+    y, add, w = rand((tokens * k, D), 1, dtype=dtype), rand((tokens, D), 2, dtype=dtype), rand((tokens, k), 3)
+    place = torch.randperm(tokens * k, generator=torch.Generator().manual_seed(4)).int()
+    for plus in (None, add):
+        on = [t if t is None else t.cuda() for t in (y, place, w, plus)]
+        out = torch.full((tokens + 1, D), 7.0, device="cuda", dtype=dtype)
+        rc = _lib.load_decoder().atma_combine_experts(*(None if t is None else t.data_ptr() for t in on), out.data_ptr(), tokens, k, D, _lib.DTYPE_CODE[dtype],
+                                                      torch.cuda.current_stream().cuda_stream)
+        assert rc == 0 and (out[tokens] == 7).all()
+        terms = y.double()[place.long()].view(tokens, k, D) * w.double()[..., None]
+        want = terms.sum(1) + (0 if plus is None else plus.double())
+        off = k * U * (terms.abs().sum(1) + (0 if plus is None else plus.double().abs()))
+        off = off + (torch.finfo(dtype).eps / 2 * (want.abs() + off) if dtype is torch.bfloat16 else 0)
+        assert ((out[:tokens].cpu().double() - want).abs() <= off).all()
