@@ -154,7 +154,9 @@ __device__ __forceinline__ void fma_chunk(uint64_t* sum, uint32_t (&r)[kChunk], 
 #pragma unroll
   for (int i = 0; i < kChunk / 2; ++i) sum[i] = fma2(pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), s2, sum[i]);
 }
-// One lane's arrival without a branch: the loads in front of it were the whole warp's.
+// One lane's arrival at the pair's first CTA, without a branch: the loads in front of it were the whole warp's.  Nothing but TMEM that has been
+// read (tcgen05.wait::ld) is handed over, so that it goes without a release, which waits for everything that the thread has in flight: 1400
+// clocks at every block of 512.
 __device__ __forceinline__ void arrive_cluster_if(bool mine, uint32_t bar) {
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %1, 0;\n\t@p mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n\t}"
                ::"r"(bar), "r"((int)mine) : "memory");

@@ -14,11 +14,6 @@ __device__ __forceinline__ uint32_t in_first(uint32_t addr) {                   
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// The same where nothing but TMEM that has been read (tcgen05.wait::ld) is handed over: without the release, which waits for everything
-// that the thread has in flight, 1400 clocks at every block of 512.
-__device__ __forceinline__ void arrive_cluster_relaxed(uint32_t bar) {
-  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
 // a tile into this CTA's memory, counted on a barrier of either
 __device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* m, uint32_t bar, int c0, int c1) {
   asm volatile(
