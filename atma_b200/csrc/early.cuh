@@ -10,7 +10,8 @@
 //
 // Steps of a few rows are launched so, whose products are this library's too.  Between a library's kernels, which neither
 // release early nor start early, it gives nothing (64 rows of Zemivik: 573 us a step without, 576 with).  The operators in 8 bits and of
-// experts, whose products are this library's at any size, pass 0 for the step's rows: always.
+// experts, whose products are this library's at any size, pass 0 for the step's rows: always; but for the residual stream's norms, which
+// go by the rows like those without 8 bits.
 //
 // One thread's release counts for its CTA.  So a kernel that takes TMEM in front of the wait shares its SM, by what it asks of shared memory
 // and of TMEM, with no more CTAs of such kernels than there are columns for: none then waits for columns of one that waits for it.

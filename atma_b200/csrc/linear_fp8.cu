@@ -17,13 +17,14 @@
 // block's wait and first load in front of the last sums (254), results by TMA (no gain, and see below).
 // The sums' 128 registers and two loads of 32 fill what a thread has: a version that spills 20 words takes 360 us.
 // Gated (65536 rows of 64 experts, 2048 x 2048) 300 us, 1.8 PFLOP/s with the gate and the rows behind the experts' ends; 1024 columns, where
-// results leave after every 8 blocks, 175 us, 1.6.
+// results leave after every 8 blocks, 175 us, 1.6, in bf16 and 220, 1.25, in fp32.
 //
 // Few rows (linear_fp8_rows_kernel): the weight's rows are the tensor core's rows, 128 a tile, and the tokens its columns, 16 to 64, so
-// that a stage is all weight.  Bound by reading that: two CTAs an SM with 100 KB of copies in flight each.  128 rows of 64 experts, 2048 x
-// 2048 gated 43 us, 6.2 TB/s; 2048 x 1024 25 us, 5.4.  Where a dense product has too few tiles for that, a cluster shares one: every CTA takes
-// its part of the columns, and each then adds up what all of them have for some of the tokens, from their shared memory and in their
-// order.  8192 x 2048: 4 rows 9.8 us, 64 rows 11.9 (20 with a token's words read one after another), 128 rows by the other kernel 12.6.
+// that a stage is all weight.  Bound by reading that: two CTAs an SM with 90 to 102 KB of copies in flight each; gated with 32 tokens 72 KB,
+// as a third stage does not fit, and gated with 64 tokens one CTA an SM with 200 KB, whose two times 64 sums and products a thread take
+// all 255 registers and spill 60 bytes.  128 rows of 64 experts, 2048 x 2048 gated 43 us, 6.2 TB/s; 2048 x 1024 25 us, 5.4.  Where a dense
+// product has too few tiles for that, a cluster shares one: every CTA takes its part of the columns, and each then adds up what all of them
+// have for some of the tokens, from their shared memory and in their order.  8192 x 2048: 4 rows 9.8 us, 64 rows 11.9 (20 with a token's words read one after another), 128 rows by the other kernel 12.6.
 //
 // Every mbarrier wait is bounded; on expiry the CTAs free their TMEM, return and leave a status word for the host.
 #include "common.cuh"

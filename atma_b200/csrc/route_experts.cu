@@ -10,8 +10,11 @@
 // grow with the logit, which is then the key itself and exact.  Weights are fp32 scores over their sum, and fp64 ones where the chosen scores
 // are below what fp32 holds: sigmoids of logits below -87, softmax beside a far larger logit that a bias or its group keeps out.
 //
-// Bound by instructions: 16384 tokens of 256 experts in 8 groups, top 8, 28 us and 9 for the order (18 MB: 2.8); 75 and 15 with a scan of the
-// lane's keys in every round and whole tokens again in fp64, which held up their CTAs by 10 us each.
+// Bound by instructions, 971 a token: 16384 tokens of 256 experts in 8 groups, top 8, 28 us and 9 for the order (18 MB: 2.8); 75 and 15 with a
+// scan of the lane's keys in every round and whole tokens again in fp64, which held up their CTAs by 10 us each.  That scan (choose) is what
+// groups of no 1, 2, 4, .. whole lanes still take, and 32 choices or more: 160 experts in 8 groups, top 6, 85 us.  A CTA of 1024 threads leaves
+// a thread 64 registers; with eight experts a lane 308 bytes of it are spilled, with sixteen 556, and most of that around the calls of
+// what few tokens need.
 // A warp holds a token's experts, V of them a lane, neighbours in neighbouring places.  Largest values come by redux over the keys as
 // ordered integers.  A NaN counts as the smallest logit, so that every choice is an expert; infinities as the largest finite values.
 //
