@@ -5,16 +5,12 @@
 // that such a row takes part in is one.
 // Rows that are given (fp8_four, fp8_one): the quotient is rounded once, to e4m3.  16-bit values over a largest one of their kind lie on, or
 // nearly on, borders between two e4m3 values in numbers (in one block of seven or so), and a quotient that is rounded to fp32 in between
-// lands on the border itself.  Norms (fp8_four_odd, fp8_one_odd): the quotient by a product with 1 / s in two words, rounded to odd, so that it
-// counts as rounded once, too; but one that is a border itself (of 24-bit values, one in 2^24 or fewer) may go either way.  Gates (.._times): a
-// product with 1 / s, which is off by less than the gate's fast exponential is.
+// lands on the border itself.  Results of fp32 arithmetic (.._times): a product with 1 / s, which is off by as little as they are.
 #pragma once
 
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <cstdint>
-
-#include "f32x2.cuh"
 
 namespace atma {
 
@@ -63,21 +59,6 @@ __device__ __forceinline__ uint32_t fp8_four(const float (&v)[4], float s) {
 __device__ __forceinline__ uint8_t fp8_one(float v, float s) {
   return __nv_cvt_float_to_fp8(fp8_quotient(v, s, fp8_inverse(s)), __NV_SATFINITE, __NV_E4M3);
 }
-// 1 / s to 2^-44 in two words; the product with them, towards zero and then odd, lies on the quotient's side of every border.
-struct Fp8Inverse { float hi, lo; };
-__device__ __forceinline__ Fp8Inverse fp8_inverse_two(float s) {
-  const float hi = fp8_inverse(s);
-  return {hi, fmaf(-hi, s, 1.0f) * hi};
-}
-__device__ __forceinline__ uint32_t fp8_two_odd(float a, float b, Fp8Inverse inv) {
-  const uint64_t v = pack2(a, b);
-  const float2 q = unpack2(fma2_rz(v, pack2(inv.hi, inv.hi), mul2(v, pack2(inv.lo, inv.lo))));
-  return fp8_two(__int_as_float(__float_as_int(q.x) | 1), __int_as_float(__float_as_int(q.y) | 1));
-}
-__device__ __forceinline__ uint32_t fp8_four_odd(const float (&v)[4], Fp8Inverse inv) {
-  return fp8_two_odd(v[0], v[1], inv) | fp8_two_odd(v[2], v[3], inv) << 16;
-}
-__device__ __forceinline__ uint8_t fp8_one_odd(float v, Fp8Inverse inv) { return (uint8_t)fp8_two_odd(v, 0.f, inv); }
 __device__ __forceinline__ uint8_t fp8_one_times(float v, float inv) { return __nv_cvt_float_to_fp8(v * inv, __NV_SATFINITE, __NV_E4M3); }
 
 }  // namespace atma

@@ -4,8 +4,10 @@
 //
 // Norms, t = x + y, h = t / sqrt(mean t^2 + eps) (offset + w): a CTA a row, which stays in registers between the sum of squares and the
 // results; scales are written block by block, a word a row, which neighbouring rows' CTAs fill up to sectors in L2.  Bound by HBM and,
-// nearly as much, by instructions (85 % of the issue slots): 32768 x 2048, bf16, two norms, one of them in bf16 too 154 us, 6.2 TB/s; 148 with
-// a product with 1 / s for the quotient, which is rounded twice; 229 with IEEE quotients and 256 threads a row.  Rows to 8 bits: 8192 x 2048 15.5 us at 1.2 GHz, 3.2 TB/s (21 with four channels a lane).
+// nearly as much, by instructions (85 % of the issue slots): 32768 x 2048, bf16, two norms, one of them in bf16 too 148 us, 6.4 TB/s; 229 with
+// IEEE quotients and 256 threads a row.  The product with 1 / s is one more fp32 rounding behind the norm's: 48 to 60 of 67 million values lie on
+// another side of a border than in 64 bits, in plain fp32 arithmetic 38 to 58; with a quotient that is rounded once 37 to 48, for 154 us.
+// Rows to 8 bits: 8192 x 2048 15.5 us at 1.2 GHz, 3.2 TB/s (21 with four channels a lane).
 // Sum of eight experts' results: 8192 x 8 x 2048 of fp32 91 us, 6.3 TB/s.
 #include "common.cuh"
 #include "early.cuh"
@@ -43,17 +45,17 @@ __device__ __forceinline__ void load_block(const T* row, int b, int lane, int wi
 template <bool kVec, bool kGiven>
 __device__ __forceinline__ void store_block(uint8_t* row, float* scale, int b, int lane, int width, const float (&v)[4]) {
   const float s = fp8_scale(warp_max_nan(max_nan(max_nan(fabsf(v[0]), fabsf(v[1])), max_nan(fabsf(v[2]), fabsf(v[3])))));
-  const Fp8Inverse inv = fp8_inverse_two(s);
+  const float inv = fp8_inverse(s);
   if (lane == 0) *scale = s;
   if constexpr (kVec) {
     const int c = b * kFp8Block + 4 * lane;
-    const uint32_t q = kGiven ? fp8_four(v, s) : fp8_four_odd(v, inv);
+    const uint32_t q = kGiven ? fp8_four(v, s) : fp8_four_times(v, inv);
     if (c < width) *reinterpret_cast<uint32_t*>(row + c) = q;
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int c = b * kFp8Block + lane + 32 * e;
-      if (c < width) row[c] = kGiven ? fp8_one(v[e], s) : fp8_one_odd(v[e], inv);
+      if (c < width) row[c] = kGiven ? fp8_one(v[e], s) : fp8_one_times(v[e], inv);
     }
   }
 }
